@@ -65,6 +65,12 @@ class Dp(C.Structure):
     _fields_ = [("global_rows", C.c_int64), ("allreduce", ALLREDUCE_FN), ("ctx", C.c_void_p)]
 
 
+class AdamwTensor(C.Structure):
+    """struct ddg_adamw_tensor (include/ddgani.h)."""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("numel", C.c_int64), ("offset", C.c_int64),
+                ("weight_decay", C.c_float), ("param_type", C.c_int32), ("grad_type", C.c_int32), ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/ddgani.h declares
 SIGNATURES = {
     "ddg_version": (C.c_int, []),
@@ -152,6 +158,25 @@ SIGNATURES = {
     "ddg_learner_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "ddg_learner_train": (C.c_int, [c_f32p, c_i32p, C.c_int64, c_f32p, c_i32p, C.c_int64, C.c_int, C.c_int, C.c_int,
                                     C.c_float, c_f32p, c_f32p, c_f32p, c_i32p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ddg_embedding": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int64, C.c_float,
+                                C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
+    "ddg_embedding_grad_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
+    "ddg_embedding_grad": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int,
+                                     C.c_float, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_size_t,
+                                     C.c_void_p]),
+    "ddg_adamw_workspace_bytes": (C.c_size_t, [C.POINTER(AdamwTensor), C.c_int]),
+    "ddg_adamw_step": (C.c_int, [C.POINTER(AdamwTensor), C.c_int, C.c_int, C.c_void_p, C.c_void_p, c_f32p, c_f32p, c_f32p,
+                                 C.c_int64, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_void_p, C.c_void_p,
+                                 C.c_size_t, C.c_void_p]),
+    "ddg_fp8_operand_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "ddg_fp8_pack_weight": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ddg_fp8_linear_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "ddg_fp8_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, c_f32p, C.c_void_p,
+                                 C.c_int, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ddg_fp8_linear_grads_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "ddg_fp8_linear_grads": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p,
+                                       C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, c_f32p, c_f32p, C.c_void_p,
+                                       C.c_size_t, C.c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,58 @@
+// Element types of the entry points that take fp32, bf16 or fp16 operands (DDG_F32 / DDG_BF16 / DDG_F16): dispatch, and
+// loads / stores of eight consecutive elements as fp32 values.
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+static inline bool ddg_type_ok(int t) { return t == DDG_F32 || t == DDG_BF16 || t == DDG_F16; }
+static inline int ddg_type_bytes(int t) { return t == DDG_F32 ? 4 : 2; }
+
+// calls f(T()) with the element type of code t, which the caller has checked with ddg_type_ok
+template <class F> static inline int ddg_with_type(int t, F &&f) {
+    switch (t) {
+        case DDG_F32: return f(float());
+        case DDG_BF16: return f(bf16_t());
+        default: return f(f16_t());
+    }
+}
+
+// n <= N consecutive elements -> fp32 (elements from n on read as 0).  A full vector is moved with the widest loads; the
+// address needs the alignment of one element only (gfx950 serves unaligned 16-byte accesses of global memory), so rows of
+// odd length take the same path.
+template <int N, class T> __device__ __forceinline__ void load_n(const T *p, int n, float (&v)[N]) {
+    if (n >= N) {
+        T t[N];
+        __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+    }
+}
+template <int N, class T> __device__ __forceinline__ void store_n(T *p, int n, const float (&v)[N]) {
+    if (n >= N) {
+        T t[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = (T)v[i];
+        __builtin_memcpy(p, t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) p[i] = (T)v[i];
+    }
+}
+
+// maximum over the 16 lanes of a DPP row, in every lane
+__device__ __forceinline__ float row16_max(float x) {
+#define DDG_DPP_MAX(ctrl)                                                                                                   \
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xF, 0xF, true)))
+    DDG_DPP_MAX(0xB1);       // quad_perm [1,0,3,2]
+    DDG_DPP_MAX(0x4E);       // quad_perm [2,3,0,1]
+    DDG_DPP_MAX(0x141);      // row_half_mirror
+    DDG_DPP_MAX(0x140);      // row_mirror
+#undef DDG_DPP_MAX
+    return x;
+}

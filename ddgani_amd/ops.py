@@ -683,3 +683,315 @@ def fd_eval(P: FdParams, X, Y, chunk_rows: int = 65536):
     check(lib().ddg_fd_eval(C.byref(P.c), _ptr(X, torch.float32), _ptr(Y, torch.int32), n, _ptr(hit), _ptr(ce),
                             ws.data_ptr(), ws.numel(), rows, _stream()), "ddg_fd_eval")
     return hit[0], ce[0]
+
+
+# ----------------------------------------------------------------------------- operators with 16-bit operands
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # DDG_F32 / DDG_BF16 / DDG_F16
+
+
+def _type(t: torch.Tensor, what: str) -> int:
+    code = _TYPE.get(t.dtype)
+    if code is None:
+        raise _lib.DdgError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _matrix(t: torch.Tensor, what: str):
+    """(pointer, elements between rows) of a 2-D device tensor whose rows are contiguous and do not overlap"""
+    if not t.is_cuda:
+        raise _lib.DdgError("ddgani_amd ops need tensors on the GPU (no CPU fallback)")
+    if t.dim() != 2:
+        raise _lib.DdgError(f"{what}: expected a matrix, got {t.dim()} dimensions")
+    rows, cols = t.shape
+    ld = t.stride(0) if rows > 1 else max(t.stride(0), cols)
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise _lib.DdgError(f"{what}: rows must be contiguous")
+    return t.data_ptr(), ld
+
+
+def _same_device(dev: torch.device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise _lib.DdgError(f"{name}: on {t.device}, expected {dev}")
+
+
+class _On:
+    """makes a tensor's device current around a call, so that the work goes to that device's current stream"""
+
+    def __init__(self, dev: torch.device):
+        self.dev = dev
+        self.guard = None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.dev.index:
+            self.guard = torch.cuda.device(self.dev)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _scratch(nbytes: int, dev: torch.device):
+    """(tensor, pointer) of a call's own workspace.  From torch's allocator and not from the per-device cache: two streams,
+    and two captured graphs, get different memory."""
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return ws, ws.data_ptr() if nbytes else None
+
+
+# ----------------------------------------------------------------------------- embedding
+def _ids(ids: torch.Tensor):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise _lib.DdgError(f"ids: expected int32 or int64, got {ids.dtype}")
+    return _ptr(ids), int(ids.dtype == torch.int64)
+
+
+def embedding(ids, table, scale: float = 1.0, out_dtype: Optional[torch.dtype] = None, out=None):
+    """ddg_embedding: scale * table[ids] -> [*ids.shape, D].  ids int32 / int64, contiguous; table [V, D] float32, bfloat16 or
+    float16 with contiguous rows (a row stride is fine).  An id outside [0, V) -- the -1 of a padded batch -- gives zeros.
+    out_dtype: of the result (default: the table's); out: a contiguous tensor, or a matrix [ids.numel(), D] with a row stride."""
+    ip, i64 = _ids(ids)
+    tp, ld = _matrix(table, "table")
+    V, D = table.shape
+    if V < 1 or D < 1:
+        raise _lib.DdgError("embedding: empty table")
+    if out is None:
+        out = torch.empty((*ids.shape, D), dtype=out_dtype or table.dtype, device=table.device)
+    elif (out_dtype is not None and out.dtype != out_dtype) or (out.shape != (*ids.shape, D) and out.shape != (ids.numel(), D)):
+        raise _lib.DdgError("embedding: out has another shape or type")
+    op, ldo = (_ptr(out), D) if out.dim() != 2 else _matrix(out, "out")
+    _same_device(table.device, ids=ids, out=out)
+    with _On(table.device):
+        check(lib().ddg_embedding(ip, i64, ids.numel(), tp, _type(table, "table"), V, D, ld, float(scale), op,
+                                  _type(out, "out"), ldo, _stream()), "ddg_embedding")
+    return out
+
+
+def embedding_grad(ids, dy, n_rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
+                   out_dtype: torch.dtype = torch.float32, out=None, accumulate: bool = False):
+    """ddg_embedding_grad: the gradient of ``embedding`` in its table, [n_rows, D]: row v is scale * the sum of dy over the
+    tokens with id v (zeros if there is none).  dy [*ids.shape, D].  Ids outside [0, n_rows) and padding_idx have no gradient.
+    accumulate: adds to ``out`` and leaves rows that no token names as they are.  Equal calls give equal bits."""
+    ip, i64 = _ids(ids)
+    n, D = ids.numel(), dy.shape[-1]
+    if dy.shape != (*ids.shape, D) and dy.shape != (n, D):
+        raise _lib.DdgError(f"embedding_grad: dy {tuple(dy.shape)} does not match ids {tuple(ids.shape)}")
+    if n_rows < 1 or D < 1:
+        raise _lib.DdgError("embedding_grad: empty table")
+    if dy.dim() == 2:
+        dp, ld = _matrix(dy, "dy")
+    else:
+        dp, ld = _ptr(dy), D
+    if out is None:
+        if accumulate:
+            raise _lib.DdgError("embedding_grad: accumulate needs out")
+        out = torch.empty((n_rows, D), dtype=out_dtype, device=dy.device)
+    elif out.shape != (n_rows, D):
+        raise _lib.DdgError(f"embedding_grad: out {tuple(out.shape)}, expected {(n_rows, D)}")
+    op, ldo = _matrix(out, "out")
+    _same_device(dy.device, ids=ids, out=out)
+    with _On(dy.device):
+        nb = lib().ddg_embedding_grad_workspace_bytes(n, D)
+        ws, wp = _scratch(nb, dy.device)
+        check(lib().ddg_embedding_grad(ip, i64, n, dp, _type(dy, "dy"), ld, int(n_rows), D, float(scale),
+                                       -1 if padding_idx is None else int(padding_idx), int(accumulate), op, _type(out, "out"),
+                                       ldo, wp, nb, _stream()), "ddg_embedding_grad")
+    return out
+
+
+# ----------------------------------------------------------------------------- dense layer in 8-bit floating point
+class Fp8Weight:
+    """A dense layer's weight [out, in] in e4m3 with one power-of-two scale for each 128 x 128 block, laid out for
+    ``linear_fp8`` and (grads=True) for ``linear_fp8_grads``; ``refresh(W)`` packs new values after an optimizer step."""
+
+    def __init__(self, W: torch.Tensor, grads: bool = True):
+        _matrix(W, "W")
+        self.out_dim, self.in_dim = W.shape
+        if self.out_dim < 1 or self.in_dim < 1:
+            raise _lib.DdgError("Fp8Weight: empty weight")
+        self.device = W.device
+        buf = lambda r, c: torch.empty(lib().ddg_fp8_operand_bytes(r, c), dtype=torch.uint8, device=W.device)
+        self.packed = buf(self.out_dim, self.in_dim)
+        self.packed_t = buf(self.in_dim, self.out_dim) if grads else None
+        self.refresh(W)
+
+    def refresh(self, W: torch.Tensor):
+        if tuple(W.shape) != (self.out_dim, self.in_dim):
+            raise _lib.DdgError(f"Fp8Weight: expected {(self.out_dim, self.in_dim)}, got {tuple(W.shape)}")
+        wp, ld = _matrix(W, "W")
+        _same_device(self.device, W=W)
+        with _On(self.device):
+            check(lib().ddg_fp8_pack_weight(wp, _type(W, "W"), ld, self.out_dim, self.in_dim, self.packed.data_ptr(),
+                                            _ptr(self.packed_t), _stream()), "ddg_fp8_pack_weight")
+
+
+def linear_fp8(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype] = None, out=None):
+    """ddg_fp8_linear: x [rows, in] times the packed weight, + bias (float32 [out]) -> [rows, out] in out_dtype (default: x's).
+    x is quantised within the call, in groups of 128 along its rows; up to 16 rows take one launch."""
+    xp, ld = _matrix(x, "x")
+    rows, inn = x.shape
+    if inn != weight.in_dim:
+        raise _lib.DdgError(f"linear_fp8: x has {inn} columns, the weight {weight.in_dim}")
+    if bias is not None and bias.shape != (weight.out_dim,):
+        raise _lib.DdgError("linear_fp8: bias has another length than the layer's output")
+    if out is None:
+        out = torch.empty((rows, weight.out_dim), dtype=out_dtype or x.dtype, device=x.device)
+    elif out.shape != (rows, weight.out_dim) or (out_dtype is not None and out.dtype != out_dtype):
+        raise _lib.DdgError("linear_fp8: out has another shape or type")
+    op, ldo = _matrix(out, "out")
+    _same_device(x.device, weight=weight.packed, bias=bias, out=out)
+    with _On(x.device):
+        nb = lib().ddg_fp8_linear_workspace_bytes(rows, inn)
+        ws, wp = _scratch(nb, x.device)
+        check(lib().ddg_fp8_linear(xp, _type(x, "x"), ld, rows, weight.packed.data_ptr(), weight.out_dim, inn,
+                                   _ptr(bias, torch.float32), op, _type(out, "out"), ldo, wp, nb, _stream()), "ddg_fp8_linear")
+    return out
+
+
+def linear_fp8_grads(dy, x, weight: Fp8Weight, want_bias: bool = False, out_dtype: Optional[torch.dtype] = None):
+    """ddg_fp8_linear_grads: gradients of ``linear_fp8`` -> (dx [rows, in] in out_dtype (default: dy's), dW [out, in] float32,
+    db [out] float32 or None).  Both products run in e4m3; db sums dy as it is."""
+    dp, ldd = _matrix(dy, "dy")
+    xp, ldx = _matrix(x, "x")
+    rows, inn = x.shape
+    if inn != weight.in_dim or dy.shape != (rows, weight.out_dim):
+        raise _lib.DdgError(f"linear_fp8_grads: dy {tuple(dy.shape)}, x {tuple(x.shape)}, weight {(weight.out_dim, inn)}")
+    if weight.packed_t is None:
+        raise _lib.DdgError("linear_fp8_grads: the weight was packed with grads=False")
+    dev, out_dim = x.device, weight.out_dim
+    _same_device(dev, dy=dy, weight=weight.packed)
+    code = _TYPE.get(out_dtype or dy.dtype)
+    if code is None:
+        raise _lib.DdgError("linear_fp8_grads: dx in float32, bfloat16 or float16")
+    new = torch.zeros if rows == 0 else torch.empty             # no rows: no products, the sums over them are zero
+    dx = torch.empty((rows, inn), dtype=out_dtype or dy.dtype, device=dev)
+    dw = new((out_dim, inn), dtype=torch.float32, device=dev)
+    db = new((out_dim,), dtype=torch.float32, device=dev) if want_bias else None
+    if rows == 0:
+        return dx, dw, db
+    with _On(dev):
+        nb = lib().ddg_fp8_linear_grads_workspace_bytes(rows, out_dim, inn)
+        ws, wp = _scratch(nb, dev)
+        check(lib().ddg_fp8_linear_grads(dp, _type(dy, "dy"), ldd, xp, _type(x, "x"), ldx, rows, weight.packed_t.data_ptr(),
+                                         out_dim, inn, dx.data_ptr(), code, inn, dw.data_ptr(), _ptr(db), wp, nb, _stream()),
+              "ddg_fp8_linear_grads")
+    return dx, dw, db
+
+
+# ----------------------------------------------------------------------------- AdamW
+ADAMW_BLOCK = 256                    # DDG_ADAMW_BLOCK
+
+
+class AdamW:
+    """AdamW over many tensors in one launch (ddg_adamw_step), states in 32 or 8 bits, gradients clipped by their global norm.
+
+    params, grads: lists of contiguous device tensors (float32, bfloat16 or float16, each of its own type), read and written
+    in place by every step; ``set_grads`` exchanges the gradients.  weight_decay: one number, or one for each tensor.
+    max_norm: clip (None: no clip); a step whose norm is not finite changes nothing and is not counted.
+    state_bits 8: e4m3 codes of m and of sqrt(v) with one float32 scale for every 256 elements (2 bytes an element, not 8).
+    masters: float32 weights behind 16-bit parameters, which become their rounding.
+
+    The state is flat: a tensor's elements begin at ``offsets[i]`` of exp_avg, exp_avg_sq (and masters, and 1 / 256 of it in
+    the scales).  The step number lives on the device, so a step captured into a graph counts on in its replays; lr and the
+    other numbers are those of the captured call."""
+
+    def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], lr: float = 1e-3, betas=(0.9, 0.999),
+                 eps: float = 1e-8, weight_decay=0.01, max_norm: Optional[float] = None, state_bits: int = 32,
+                 masters: bool = False):
+        self.params = list(params)
+        if not self.params:
+            raise _lib.DdgError("AdamW: no tensors")
+        if state_bits not in (8, 32):
+            raise _lib.DdgError(f"AdamW: states in 8 or 32 bits, not {state_bits}")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1) or not eps >= 0 or not lr >= 0:
+            raise _lib.DdgError("AdamW: betas in [0, 1), eps >= 0, lr >= 0")
+        if max_norm is not None and not max_norm > 0:
+            raise _lib.DdgError("AdamW: max_norm > 0, or None")
+        self.lr, self.betas, self.eps, self.max_norm, self.state_bits = lr, tuple(betas), eps, max_norm, state_bits
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(self.params)
+        if len(decay) != len(self.params):
+            raise _lib.DdgError("AdamW: one weight_decay, or one for each tensor")
+        self.weight_decay = [float(w) for w in decay]
+        self.device = dev = self.params[0].device
+        spans = sorted((_ptr(p), p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise _lib.DdgError("AdamW: parameters share memory")
+        self.offsets, total = [], 0
+        for p in self.params:
+            self.offsets.append(total)
+            total += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
+        self.state_len = total
+        zeros = lambda n, dt: torch.zeros(n, dtype=dt, device=dev)
+        code = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        _type_of = [_type(p, "params") for p in self.params]
+        _same_device(dev, **{f"params[{i}]": p for i, p in enumerate(self.params)})
+        # (zeros as bytes: a fill kernel is not needed for every element type)
+        self.exp_avg = zeros(total * code.itemsize, torch.uint8).view(code)
+        self.exp_avg_sq = zeros(total * code.itemsize, torch.uint8).view(code)
+        self.exp_avg_scale = zeros(total // ADAMW_BLOCK, torch.float32) if state_bits == 8 else None
+        self.exp_avg_sq_scale = zeros(total // ADAMW_BLOCK, torch.float32) if state_bits == 8 else None
+        self.masters = zeros(total, torch.float32) if masters else None
+        if masters:
+            for p, o in zip(self.params, self.offsets):
+                self.masters[o:o + p.numel()] = p.detach().reshape(-1)
+        self.control = zeros(8, torch.int64)                 # DDG_ADAMW_CONTROL_BYTES
+        self.step_count = self.control[:1]
+        self.norm = self.control.view(torch.float32)[2:3]
+        self._t = (_lib.AdamwTensor * len(self.params))()
+        for i, p in enumerate(self.params):
+            self._t[i] = _lib.AdamwTensor(_ptr(p), None, p.numel(), self.offsets[i], self.weight_decay[i], _type_of[i], 0, 0)
+        self._ws = None
+        self.set_grads(grads)
+
+    def set_grads(self, grads: Sequence[torch.Tensor]):
+        """the gradients that the following steps read, one for each parameter"""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise _lib.DdgError("AdamW: one gradient for each parameter")
+        for p, g in zip(self.params, grads):
+            if g.shape != p.shape:
+                raise _lib.DdgError(f"AdamW: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
+        ptr = [(_ptr(g), _type(g, "grads")) for g in grads]
+        _same_device(self.device, **{f"grads[{i}]": g for i, g in enumerate(grads)})
+        for t, (p, code) in zip(self._t, ptr):
+            t.grad, t.grad_type = p, code
+        self.grads = grads
+        if self.max_norm is not None and self._ws is None:
+            self._ws = torch.empty(lib().ddg_adamw_workspace_bytes(self._t, len(self._t)), dtype=torch.uint8, device=self.device)
+
+    def step(self, lr: Optional[float] = None):
+        """one step; lr: for this and the following steps.  -> the gradients' norm before the clip, a float32 [1] device tensor
+        that the next step overwrites (None without max_norm)"""
+        if lr is not None:
+            self.lr = lr
+        clip = self.max_norm is not None
+        with _On(self.device):
+            check(lib().ddg_adamw_step(self._t, len(self._t), self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                                       _ptr(self.exp_avg_scale), _ptr(self.exp_avg_sq_scale), _ptr(self.masters), self.state_len,
+                                       self.lr, self.betas[0], self.betas[1], self.eps, self.max_norm if clip else 0.0,
+                                       self.control.data_ptr(), _ptr(self._ws), self._ws.numel() if clip else 0, _stream()),
+                  "ddg_adamw_step")
+        return self.norm if clip else None
+
+    def state_dict(self):
+        """the handle's own tensors: step [1], exp_avg, exp_avg_sq and, where there are any, the scales and the masters"""
+        sd = dict(step=self.step_count, exp_avg=self.exp_avg, exp_avg_sq=self.exp_avg_sq)
+        if self.state_bits == 8:
+            sd.update(exp_avg_scale=self.exp_avg_scale, exp_avg_sq_scale=self.exp_avg_sq_scale)
+        if self.masters is not None:
+            sd["masters"] = self.masters
+        return sd
+
+    def load_state_dict(self, sd):
+        """copies a state saved by state_dict() of a handle with the same tensors, state_bits and masters"""
+        own = self.state_dict()
+        if sd.keys() != own.keys():
+            raise _lib.DdgError(f"AdamW: state has {sorted(sd)}, expected {sorted(own)}")
+        for k, t in own.items():
+            if k != "step" and (sd[k].shape != t.shape or sd[k].dtype != t.dtype):
+                raise _lib.DdgError(f"AdamW: {k} is {sd[k].dtype} {tuple(sd[k].shape)}, expected {t.dtype} {tuple(t.shape)}")
+        for k, t in own.items():
+            if k == "step":
+                t.fill_(int(sd[k]))
+            else:
+                t.view(torch.uint8).copy_(sd[k].view(torch.uint8))

@@ -41,6 +41,11 @@ extern "C" {
 #define DDG_E_COLLECTIVE (-6) /* the caller's all-reduce callback reported a failure            */
 #define DDG_E_SCRATCH_LIMIT (-5) /* input larger than the static scratch of a *_static entry point */
 
+/* element types of the entry points that take 16-bit operands */
+#define DDG_F32 0
+#define DDG_BF16 1
+#define DDG_F16 2
+
 #define DDG_MAX_D 256         /* widest encoded table the attention kernels are built for   */
 #define DDG_MAX_TOPK_REG 30   /* absolute k up to this uses the in-register selection       */
 
@@ -526,6 +531,85 @@ int ddg_encode_table(const double *vals, const int32_t *offsets_dev, const uint8
 int ddg_decode_table(const float *code, const uint8_t *m, const double *obs, const int32_t *offsets_dev,
                      const uint8_t *is_cat_dev, const double *dec_K, const double *dec_min, const uint8_t *dec_f32,
                      const double *pos_value, double *out, int64_t N, int C, int D, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Table lookup with a scale, and its gradient.  No reference counterpart (the reference one-hot
+ * encodes every category in front of a dense layer, utils/util.py:52-78).
+ *   y[i,:]  = scale * table[ids[i],:]
+ *   dE[v,:] = (accumulate ? dE[v,:] : 0) + scale * sum over {i: ids[i] = v} of dy[i,:]
+ * ids: int32 (ids_64 = 0) or int64 [n]; an id outside [0, V) reads as a row of zeros and has no
+ * gradient; padding_idx (-1: none) reads its row and has no gradient.  *_type: DDG_F32 / BF16 / F16,
+ * independent of each other; ld_*: elements between rows.  Sums in fp32, one rounding at the end, in
+ * an order that depends on the arguments alone: equal calls give equal bits.  With accumulate, rows
+ * that no id names are left as they are; without, they become zero.
+ * V <= 2^31 - 1 (gradient: 2^31 - 2), n <= 2^31 - 1 (gradient).
+ * ------------------------------------------------------------------------------------- */
+int ddg_embedding(const void *ids, int ids_64, int64_t n, const void *table, int table_type, int64_t V, int D,
+                  int64_t ld_table, float scale, void *out, int out_type, int64_t ld_out, void *stream);
+size_t ddg_embedding_grad_workspace_bytes(int64_t n, int D);
+int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const void *dy, int dy_type, int64_t ld_dy, int64_t V,
+                       int D, float scale, int64_t padding_idx, int accumulate, void *out, int out_type,
+                       int64_t ld_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * AdamW over many tensors at once (decoupled weight decay; ddg_adam_step is Adam with coupled L2),
+ * states in 32 or 8 bits, gradients clipped by their global norm.  No reference counterpart.
+ *   c = min(1, max_norm / (|g| + 1e-6))  (max_norm <= 0: no clip);  g' = c g
+ *   m += (1 - b1)(g' - m);  v = b2 v + (1 - b2) g'^2
+ *   w = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * States are flat buffers of state_len elements; a tensor's numel elements begin at `offset`, a
+ * multiple of DDG_ADAMW_BLOCK, and tensors do not overlap in them.
+ * state_bits 32: exp_avg, exp_avg_sq fp32 (m, v); the scales are not read.
+ * state_bits 8: e4m3 codes of m and of sqrt(v), one fp32 scale for every DDG_ADAMW_BLOCK elements
+ *   (scale[offset / DDG_ADAMW_BLOCK + block]); value = code * scale.  m to nearest; sqrt(v) by a
+ *   dither that is a function of (element, step), so that equal calls give equal bits.
+ * masters (may be NULL): fp32 weights of the 16-bit parameters, flat like the states; the parameter
+ *   becomes the rounding of its master.  fp32 parameters do not use it.
+ * control: DDG_ADAMW_CONTROL_BYTES of device memory, zeroed by the caller before the first step: int64 step count at byte 0,
+ *   float norm of the last step at byte 8 (max_norm > 0).  The step number advances on the device,
+ *   so a captured graph may be replayed.  If the norm is not finite nothing changes but `norm`.
+ * tensors: HOST array, read before the call returns.  workspace: only for max_norm > 0.
+ * ------------------------------------------------------------------------------------- */
+#define DDG_ADAMW_BLOCK 256
+#define DDG_ADAMW_CONTROL_BYTES 64
+typedef struct ddg_adamw_tensor {
+    void *param;
+    const void *grad;
+    int64_t numel, offset;
+    float weight_decay;
+    int32_t param_type, grad_type;      /* DDG_F32 / DDG_BF16 / DDG_F16 */
+    int32_t reserved;
+} ddg_adamw_tensor;
+size_t ddg_adamw_workspace_bytes(const ddg_adamw_tensor *tensors, int n_tensors);
+int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, int state_bits, void *exp_avg, void *exp_avg_sq,
+                   float *exp_avg_scale, float *exp_avg_sq_scale, float *masters, int64_t state_len, double lr,
+                   double beta1, double beta2, double eps, double max_norm, void *control, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Dense layer in 8-bit floating point (e4m3, values up to 448), one power-of-two scale for each
+ * block of 128: the layer of ddg_linear (Generator_x0.forward, model/Diffusion.py:179-187) without
+ * its prologues, for throughput.  Products exact, sums in fp32.
+ *   Y = Q(X) Q(W)^T + bias         X in groups of 128 along a row, W [out, in] in 128 x 128 blocks
+ *   dX = Q(dY) Q(W)                dY in groups along a row
+ *   dW = Q'(dY)^T Q'(X)            groups of 128 along the batch;  db = column sums of dY in fp32
+ * A block's scale is the smallest power of two that brings its largest magnitude to 448 or below;
+ * a block whose largest magnitude is below 2^-100 counts as zeros.  Infinities and NaN give NaN.
+ * Packed operand [rows, cols]: ddg_fp8_operand_bytes(rows, cols) bytes, aligned to 256.
+ * ddg_fp8_pack_weight: W -> packed [out, in] and, for the gradients, packed_t [in, out] (may be NULL).
+ * dx and db may not be NULL / may be NULL.  A workspace is aligned to 256.
+ * ------------------------------------------------------------------------------------- */
+size_t ddg_fp8_operand_bytes(int64_t rows, int64_t cols);
+int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t out, int64_t in, void *packed, void *packed_t,
+                        void *stream);
+size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t in);
+int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t rows, const void *packed_w, int64_t out, int64_t in,
+                   const float *bias, void *y, int y_type, int64_t ld_y, void *workspace, size_t workspace_bytes,
+                   void *stream);
+size_t ddg_fp8_linear_grads_workspace_bytes(int64_t rows, int64_t out, int64_t in);
+int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, const void *x, int x_type, int64_t ld_x,
+                         int64_t rows, const void *packed_wt, int64_t out, int64_t in, void *dx, int dx_type,
+                         int64_t ld_dx, float *dw, float *db, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
