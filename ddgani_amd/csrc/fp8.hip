@@ -19,13 +19,15 @@
 //
 // Packed operand of `rows` rows and a reduction of `cols`: codes [rows][colsp] (colsp = cols rounded up to 128, zeros
 // behind cols), then from the next multiple of 256 bytes the scales as biased exponents (2^(e - 127)), four consecutive
-// blocks in one word: word [block / 4][row], byte block % 4.  The 16 rows of a matrix tile are 16 consecutive words.
+// blocks in one word: word [block / 4][row], byte block % 4.  The 16 rows of a matrix tile are 16 consecutive words.  1 KB
+// behind the scales belongs to the operand too: a workgroup reads whole 256-row pieces of them.
 #include <type_traits>
 #include "types.h"
 
 #define F8_BLOCK 128
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 static __host__ __device__ __forceinline__ int64_t f8_pad(int64_t cols) { return (cols + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK; }
@@ -33,7 +35,7 @@ static __host__ __device__ __forceinline__ size_t f8_codes_bytes(int64_t rows, i
     return ((size_t)rows * f8_pad(cols) + 255) & ~(size_t)255;
 }
 static inline size_t f8_scale_bytes(int64_t rows, int64_t cols) {
-    return (((size_t)rows * ((f8_pad(cols) / F8_BLOCK + 3) / 4) * 4) + 255) & ~(size_t)255;
+    return (((size_t)rows * ((f8_pad(cols) / F8_BLOCK + 3) / 4) * 4) + 1024 + 255) & ~(size_t)255;
 }
 struct F8Operand {
     uint8_t *q, *s;
@@ -201,14 +203,34 @@ __global__ __launch_bounds__(256) void k_f8_colsum(const float *__restrict__ par
 // ---------------------------------------------------------------------------------------------
 // product of two packed operands: C[m, n] = sum over k of A[m, k] B[n, k]
 // ---------------------------------------------------------------------------------------------
-// LDS image of a stage: rows of 128 bytes (one block of the reduction), whose eight 16-byte pieces are exchanged by
-// piece ^ (row / 2 % 8): a quarter wave that reads one piece of 16 consecutive rows touches all 64 banks once.  The
-// copy into LDS writes linearly, so the exchange is applied to the global address.
-__device__ __forceinline__ int f8_piece(int row, int piece) { return piece ^ ((row >> 1) & 7); }
+// A workgroup owns BM x BN of the result, a wave MT x NT tiles of 16 x 16; one block of the reduction is a stage.
+//
+// LDS image of a stage: rows of 128 bytes, whose eight 16-byte pieces are exchanged by f8_swap(row).  A 16-byte read is served
+// in groups of 16 lanes, 0-3 + 12-15 + 20-27 and so on; with a fragment's lanes (row lane % 16, pieces lane / 16 * 2 and + 1) such a
+// group asks for one piece of eight rows and for another one of the other eight, and f8_swap puts all 16 into different
+// banks.  (row / 2 % 8 alone, right for 16 consecutive lanes, had every read take twice its time.)  The copy from global
+// memory straight to LDS writes linearly, so the exchange is applied to the global address.  The scale words of four stages
+// lie behind the two stages.
+//
+// One barrier per stage, placed before the last column of tiles of stage k: by then every fragment of stage k has been read,
+// so its buffer takes stage k + 2 while stage k + 1, whose copy was issued one stage ago, has landed; its fragments are read
+// between the matrix instructions of that last column, each register right after its last use.
+template <int MT, int NT, int WM, int WN> struct F8Shape {
+    static constexpr int WAVES = WM * WN, BM = MT * 16 * WM, BN = NT * 16 * WN, ROWS = BM + BN, LOADS = ROWS / 8 / WAVES,
+                         LOADS_A = BM / 8 / WAVES, STAGE = ROWS * F8_BLOCK, STAGES = 2 * STAGE + 2 * ROWS * 4;
+    // the finished tile of a wave: rows of NT * 16 elements and 16 bytes, so that rows start in different banks
+    static constexpr int PITCH(int bytes) { return NT * 16 * bytes + 16; }
+    static constexpr int OUT(int bytes) { return MT * 16 * PITCH(bytes); }
+    static constexpr int LDS(int bytes) { return STAGES > WAVES * OUT(bytes) ? STAGES : WAVES * OUT(bytes); }
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && ROWS == 64 * WAVES && BM % 64 == 0,
+                  "whole copies: eight rows of codes, 64 rows of scale words per wave");
+};
+
+__device__ __forceinline__ int f8_swap(int row) { return ((row >> 1) & 7) ^ ((((row >> 2) ^ (row >> 3)) & 1) << 1); }
 
 // 32 codes of a lane -> the operands of four bf16 instructions, multiplied by the scale of biased exponent e
 __device__ __forceinline__ void f8_expand(const i32x8 &f, uint32_t e, bf16x8 (&o)[4]) {
-    const float s = __builtin_bit_cast(float, (e & 0xFF) << 23);
+    const float s = __builtin_bit_cast(float, e << 23);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[i], s, false);
@@ -220,116 +242,171 @@ __device__ __forceinline__ void f8_expand(const i32x8 &f, uint32_t e, bf16x8 (&o
     }
 }
 
-template <int BM, int BN, int WM, int WN, bool EXPAND, class TO>
-__global__ __launch_bounds__(64 * WM * WN) void k_f8_gemm(const uint8_t *__restrict__ A, const uint32_t *__restrict__ As, int64_t M,
-                                                          const uint8_t *__restrict__ B, const uint32_t *__restrict__ Bs, int64_t N,
-                                                          int64_t kp, const float *__restrict__ bias, TO *__restrict__ C, int64_t ldc,
-                                                          int64_t tiles_m) {
-    constexpr int WAVES = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, ROWS = BM + BN, LOADS = ROWS / 8 / WAVES;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][ROWS * F8_BLOCK];
+// copies 16 (4) bytes per lane from base + off to LDS address dst + lane * 16 (4).  The compiler does not wait for these
+// copies in front of the LDS reads below (the address goes through an integer, and the reads are of plain vector types):
+// the barriers do
+__device__ __forceinline__ void f8_copy16(const void *base, uint32_t off, uint32_t dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)((const char *)base + off),
+                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+__device__ __forceinline__ void f8_copy4(const void *base, uint32_t off, uint32_t dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)((const char *)base + off),
+                                     (__attribute__((address_space(3))) void *)dst, 4, 0, 0);
+}
+
+template <int MT, int NT, int WM, int WN, bool EXPAND, class TO>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__restrict__ A, const uint32_t *__restrict__ As,
+                                                             int64_t M, const uint8_t *__restrict__ B,
+                                                             const uint32_t *__restrict__ Bs, int64_t N, int64_t kp,
+                                                             const float *__restrict__ bias, TO *__restrict__ C, int64_t ldc,
+                                                             uint32_t tiles_m, uint32_t tiles_n) {
+    using S = F8Shape<MT, NT, WM, WN>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;
-    const int64_t m0 = tm * BM, n0 = tn * BN;
-    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    // Tiles in bands of 8 along m, and every XCD (workgroups go round the eight XCDs) a consecutive run of them: the 32 or
+    // more workgroups that share an L2 work on a few rows and columns of tiles
+    const uint32_t tiles = tiles_m * tiles_n, q = tiles / 8, rest = tiles % 8, xcd = blockIdx.x % 8;
+    const uint32_t t = xcd * q + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    const uint32_t band = t / (8 * tiles_n), in_band = t - band * 8 * tiles_n;
+    const uint32_t height = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+    const int64_t m0 = (int64_t)(band * 8 + in_band % height) * S::BM, n0 = (int64_t)(in_band / height) * S::BN;
+    const int wm = (wave % WM) * (MT * 16), wn = (wave / WM) * (NT * 16);
     const int nk = (int)(kp / F8_BLOCK);
 
-    // this wave's copies: 8 rows each, rows behind the end repeat the last one
-    const uint8_t *src[LOADS];
+    const uint8_t *const a0 = A + m0 * kp, *const b0 = B + n0 * kp;
+    const int64_t rows_a = M - m0, rows_b = N - n0;
+    uint32_t off[S::LOADS];                             // rows behind the end repeat the last one
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int row = (i * WAVES + wave) * 8 + (lane >> 3), piece = f8_piece(row, lane & 7);
-        if (row < BM) {
-            const int64_t r = m0 + row < M ? m0 + row : M - 1;
-            src[i] = A + r * kp + piece * 16;
-        } else {
-            const int64_t r = n0 + row - BM < N ? n0 + row - BM : N - 1;
-            src[i] = B + r * kp + piece * 16;
-        }
+    for (int i = 0; i < S::LOADS; ++i) {
+        const int in = (i * S::WAVES + wave) * 8 + (lane >> 3), row = i < S::LOADS_A ? in : in - S::BM;
+        const int64_t last = (i < S::LOADS_A ? rows_a : rows_b) - 1;
+        off[i] = (uint32_t)(row < last ? row : last) * (uint32_t)kp + (((lane & 7) ^ f8_swap(in)) * 16);
     }
+    const bool scale_a = wave * 64 < S::BM;
+    const uint32_t *const s0 = scale_a ? As + m0 + wave * 64 : Bs + n0 + (wave * 64 - S::BM);
+    const int64_t s_rows = scale_a ? M : N;
+    // stage k to buffer buf.  No branch in here: the compiler would move matrix instructions across it.  Scale words are
+    // copied with each of their four stages (the same bytes over themselves)
     auto copy = [&](int k, int buf) {
+        const uint32_t dst = lds0 + buf * S::STAGE + wave * 8 * F8_BLOCK;
+        const uint8_t *a = a0 + (int64_t)k * F8_BLOCK, *b = b0 + (int64_t)k * F8_BLOCK;
+        asm("" : "+s"(a), "+s"(b));                     // scalar bases and 32-bit offsets: one register per copy and lane
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[i] + (int64_t)k * F8_BLOCK),
-                                             (__attribute__((address_space(3))) void *)&lds[buf][(i * WAVES + wave) * 8 * F8_BLOCK],
-                                             16, 0, 0);
+        for (int i = 0; i < S::LOADS; ++i) {
+            uint32_t o = off[i];
+            asm("" : "+v"(o));
+            f8_copy16(i < S::LOADS_A ? a : b, o, dst + i * S::WAVES * 8 * F8_BLOCK);
+        }
+        // (an operand's scales are followed by 1 KB that may be read)
+        const uint32_t *sc = s0 + (k >> 2) * s_rows;
+        asm("" : "+s"(sc));
+        f8_copy4(sc, lane * 4, lds0 + 2 * S::STAGE + ((k >> 2) & 1) * (S::ROWS * 4) + wave * 256);
     };
-    // this lane's scale words: operand row lane % 16 of every 16-row tile
-    const uint32_t *sa[MT], *sb[NT];
+    // this lane's two pieces of a fragment (row lane % 16 of a tile, 32 codes of the block) and its scale, for the wave's
+    // first tile of either operand; the other tiles lie at constant distances
+    const int r16 = lane & 15, swap = f8_swap(r16), g2 = (lane >> 4) * 2;
+    const uint8_t *const lo_a = lds + (wm + r16) * F8_BLOCK + (g2 ^ swap) * 16, *const hi_a = lds + (wm + r16) * F8_BLOCK + ((g2 + 1) ^ swap) * 16;
+    const uint8_t *const lo_b = lo_a + (S::BM + wn - wm) * F8_BLOCK, *const hi_b = hi_a + (S::BM + wn - wm) * F8_BLOCK;
+    const uint8_t *const sc_a = lds + 2 * S::STAGE + (wm + r16) * 4, *const sc_b = sc_a + (S::BM + wn - wm) * 4;
+    auto frag = [&](const uint8_t *lo, const uint8_t *hi, int k, int tile) {
+        const i32x4 x = *(const i32x4 *)(lo + (k & 1) * S::STAGE + tile * (16 * F8_BLOCK));
+        const i32x4 y = *(const i32x4 *)(hi + (k & 1) * S::STAGE + tile * (16 * F8_BLOCK));
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto scale = [&](const uint8_t *sc, int k, int tile) -> uint32_t {
+        return *(sc + (((k >> 2) & 1) * (S::ROWS * 4) + (k & 3)) + tile * 64);
+    };
+
+    f32x4 acc[NT][MT] = {};
+    i32x8 fa[MT], fb;
+    uint32_t ea[MT], eb;
+    copy(0, 0);
+    copy(nk > 1 ? 1 : 0, 1);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int64_t r = m0 + wm + i * 16 + (lane & 15);
-        sa[i] = As + (r < M ? r : M - 1);
+        fa[i] = frag(lo_a, hi_a, 0, i);
+        ea[i] = scale(sc_a, 0, i);
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int64_t r = n0 + wn + j * 16 + (lane & 15);
-        sb[j] = Bs + (r < N ? r : N - 1);
-    }
-    uint32_t ea[MT], eb[NT];
-    f32x4 acc[NT][MT] = {};
-    auto frag = [&](const uint8_t *base, int row) {
-        i32x8 f;
-        const uint8_t *p = base + row * F8_BLOCK;
-        const int4 lo = *(const int4 *)(p + f8_piece(row, (lane >> 4) * 2) * 16), hi = *(const int4 *)(p + f8_piece(row, (lane >> 4) * 2 + 1) * 16);
-        f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
-        f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
-        return f;
-    };
-    copy(0, 0);
+    fb = frag(lo_b, hi_b, 0, 0);
+    eb = scale(sc_b, 0, 0);
     for (int k = 0; k < nk; ++k) {
-        __syncthreads();                                // stage k has landed, stage k - 1 has been read
-        if (k + 1 < nk) copy(k + 1, (k + 1) & 1);
-        if ((k & 3) == 0) {
+        bf16x8 xa[EXPAND ? MT : 1][4];
+        if constexpr (EXPAND)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) ea[i] = sa[i][(int64_t)(k >> 2) * M];
+            for (int i = 0; i < MT; ++i) f8_expand(fa[i], ea[i], xa[i]);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) eb[j] = sb[j][(int64_t)(k >> 2) * N];
-        }
-        const uint8_t *la = lds[k & 1], *lb = lds[k & 1] + BM * F8_BLOCK;
-        i32x8 fa[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) fa[i] = frag(la, wm + i * 16 + (lane & 15));
-        const int sh = (k & 3) * 8;
-        // first operand of the instructions: rows of the result = n, so that a lane gets four consecutive n
-        if constexpr (EXPAND) {
-            bf16x8 xa[MT][4];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) f8_expand(fa[i], ea[i] >> sh, xa[i]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                bf16x8 xb[4];
-                f8_expand(frag(lb, wn + j * 16 + (lane & 15)), eb[j] >> sh, xb);
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-                        acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[i][t], acc[j][i], 0, 0, 0);
+        for (int j = 0; j < NT; ++j) {
+            bf16x8 xb[4];
+            if constexpr (EXPAND) f8_expand(fb, eb, xb);
+            const i32x8 cb = fb;
+            const uint32_t ce = eb;
+            if (j + 1 < NT) {
+                fb = frag(lo_b, hi_b, k, j + 1);
+                eb = scale(sc_b, k, j + 1);
+            } else {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                copy(k + 2 < nk ? k + 2 : nk - 1, k & 1);
+                fb = frag(lo_b, hi_b, k + 1, 0);        // (behind the last stage: read and not used)
+                eb = scale(sc_b, k + 1, 0);
             }
-        } else {
+            __builtin_amdgcn_sched_barrier(0);
+            // first operand of the instructions: rows of the result = n, so that a lane gets four consecutive n
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const i32x8 fb = frag(lb, wn + j * 16 + (lane & 15));
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (EXPAND) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa[i], acc[j][i], 0, 0, 0,
-                                                                                (int)(eb[j] >> sh), 0, (int)(ea[i] >> sh));
+                    for (int u = 0; u < 4; ++u) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[u], xa[i][u], acc[j][i], 0, 0, 0);
+                } else {
+                    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(cb, fa[i], acc[j][i], 0, 0, 0, (int)ce, 0,
+                                                                                (int)ea[i]);
+                }
+                if (j + 1 == NT) {
+                    fa[i] = frag(lo_a, hi_a, k + 1, i);
+                    ea[i] = scale(sc_a, k + 1, i);
+                    __builtin_amdgcn_sched_barrier(0);  // not earlier: the register is in use until here
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // The copies behind the last stage end here, and the stages' memory becomes the waves' own: a wave turns its tile around in
+    // LDS, so that it is written in whole rows of NT * 16 elements (128 bytes and more), not in pieces of four
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    uint8_t *const own = lds + wave * S::OUT(sizeof(TO));
+    constexpr int PITCH = S::PITCH(sizeof(TO)), VEC = 16 / sizeof(TO), LPR = NT * 16 / VEC, RPI = 64 / LPR;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int64_t n = n0 + wn + j * 16 + (lane >> 4) * 4;
-        const int left = N - n >= 4 ? 4 : N > n ? (int)(N - n) : 0;
         float b[4] = {};
-        if (bias) load_n<4>(bias + n, left, b);
+        if (bias) load_n<4>(bias + n, N - n >= 4 ? 4 : N > n ? (int)(N - n) : 0, b);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const int64_t m = m0 + wm + i * 16 + (lane & 15);
-            if (m >= M) continue;
-            float v[4];
+            typedef TO out4 __attribute__((ext_vector_type(4)));
+            out4 v;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) v[t] = acc[j][i][t] + b[t];
-            store_n<4>(C + m * ldc + n, left, v);
+            for (int u = 0; u < 4; ++u) v[u] = (TO)(acc[j][i][u] + b[u]);
+            *(out4 *)(own + (i * 16 + r16) * PITCH + (j * 16 + (lane >> 4) * 4) * sizeof(TO)) = v;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();                    // (a wave's LDS accesses stay in order)
+    const int64_t n = n0 + wn + (lane % LPR) * VEC;
+    const int left = N - n >= VEC ? VEC : N > n ? (int)(N - n) : 0;
+#pragma unroll 4
+    for (int i = 0; i < MT * 16; i += RPI) {
+        const int row = i + lane / LPR;
+        const int64_t m = m0 + wm + row;
+        if (m >= M) continue;
+        TO v[VEC];
+        __builtin_memcpy(v, __builtin_assume_aligned(own + row * PITCH + (lane % LPR) * 16, 16), 16);
+        TO *o = C + m * ldc + n;
+        if (left == VEC) {
+            __builtin_memcpy(o, v, 16);
+        } else {
+#pragma unroll
+            for (int u = 0; u < VEC; ++u)
+                if (u < left) o[u] = v[u];
         }
     }
 }
@@ -368,7 +445,7 @@ __global__ __launch_bounds__(64 * F8_SKW) void k_f8_skinny(const TX *__restrict_
             fa[i] = (int)f8_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
         bf16x8 xa[4], xb[4];
         f8_expand(fa, e, xa);
-        f8_expand(fb, eb, xb);
+        f8_expand(fb, eb & 0xFF, xb);
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
     }
@@ -422,25 +499,32 @@ static int f8_pack_tile(const void *x, int type, int64_t ld, int64_t rows, int64
     });
 }
 
+// reductions are addressed with 32-bit offsets within a workgroup's 256 rows
+#define F8_MAX_REDUCTION ((int64_t)1 << 24)
+
 static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int type, int64_t ldc, hipStream_t s) {
+    if (f8_pad(a.cols) >= F8_MAX_REDUCTION) return DDG_E_UNSUPPORTED;
     return ddg_with_type(type, [&](auto t) {
         using TO = decltype(t);
         constexpr bool EXPAND = !std::is_same<TO, bf16_t>::value;
-        auto go = [&](auto bm, auto bn, auto wm, auto wn) {
-            constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
-            const int64_t tm = ceil_div64(a.rows, BM), tn = ceil_div64(b.rows, BN);
-            if (tm * tn > 0x7FFFFFFF) return (int)DDG_E_UNSUPPORTED;
-            k_f8_gemm<BM, BN, WM, WN, EXPAND, TO><<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(
-                a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s, b.rows, f8_pad(a.cols), bias, (TO *)c, ldc, tm);
+        auto go = [&](auto mt, auto nt, auto wm, auto wn) {
+            constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+            using S = F8Shape<MT, NT, WM, WN>;
+            const int64_t tm = ceil_div64(a.rows, S::BM), tn = ceil_div64(b.rows, S::BN);
+            if (tm * tn > 0x0FFFFFFF) return (int)DDG_E_UNSUPPORTED;
+            const auto kernel = k_f8_gemm<MT, NT, WM, WN, EXPAND, TO>;
+            if (hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    S::LDS(sizeof(TO))) != hipSuccess)
+                return (int)DDG_E_LAUNCH;
+            kernel<<<(unsigned)(tm * tn), 64 * WM * WN, S::LDS(sizeof(TO)), s>>>(a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s,
+                                                                     b.rows, f8_pad(a.cols), bias, (TO *)c, ldc, (uint32_t)tm,
+                                                                     (uint32_t)tn);
             DDG_CHECK_LAUNCH();
             return (int)DDG_OK;
         };
-        if constexpr (EXPAND) {
-            return go(Int<128>(), Int<128>(), Int<2>(), Int<2>());
-        } else {
-            if (ceil_div64(a.rows, 256) * ceil_div64(b.rows, 256) >= 192) return go(Int<256>(), Int<256>(), Int<2>(), Int<4>());
-            return go(Int<128>(), Int<128>(), Int<2>(), Int<2>());
-        }
+        if constexpr (!EXPAND)
+            if (ceil_div64(a.rows, 256) * ceil_div64(b.rows, 256) >= 192) return go(Int<8>(), Int<4>(), Int<2>(), Int<4>());
+        return go(Int<4>(), Int<4>(), Int<2>(), Int<2>());
     });
 }
 
