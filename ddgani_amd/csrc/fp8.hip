@@ -213,8 +213,10 @@ __global__ __launch_bounds__(256) void k_f8_colsum(const float *__restrict__ par
 // lie behind the two stages.
 //
 // One barrier per stage, placed before the last column of tiles of stage k: by then every fragment of stage k has been read,
-// so its buffer takes stage k + 2 while stage k + 1, whose copy was issued one stage ago, has landed; its fragments are read
-// between the matrix instructions of that last column, each register right after its last use.
+// so its buffer takes stage k + 2, and stage k + 1 has landed, whose fragments are read between the matrix instructions of
+// that last column, each register right after its last use.  The copies of a stage are issued one by one between the matrix
+// instructions of two columns: issued in a row they hold up the instructions behind them, as a CU takes about 64 bytes of
+// them a cycle.
 template <int MT, int NT, int WM, int WN> struct F8Shape {
     static constexpr int WAVES = WM * WN, BM = MT * 16 * WM, BN = NT * 16 * WN, ROWS = BM + BN, LOADS = ROWS / 8 / WAVES,
                          LOADS_A = BM / 8 / WAVES, STAGE = ROWS * F8_BLOCK, STAGES = 2 * STAGE + 2 * ROWS * 4;
@@ -286,22 +288,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__re
     const bool scale_a = wave * 64 < S::BM;
     const uint32_t *const s0 = scale_a ? As + m0 + wave * 64 : Bs + n0 + (wave * 64 - S::BM);
     const int64_t s_rows = scale_a ? M : N;
-    // stage k to buffer buf.  No branch in here: the compiler would move matrix instructions across it.  Scale words are
-    // copied with each of their four stages (the same bytes over themselves)
-    auto copy = [&](int k, int buf) {
-        const uint32_t dst = lds0 + buf * S::STAGE + wave * 8 * F8_BLOCK;
-        const uint8_t *a = a0 + (int64_t)k * F8_BLOCK, *b = b0 + (int64_t)k * F8_BLOCK;
-        asm("" : "+s"(a), "+s"(b));                     // scalar bases and 32-bit offsets: one register per copy and lane
-#pragma unroll
-        for (int i = 0; i < S::LOADS; ++i) {
+    // piece i of stage k to buffer buf; the scale words are piece LOADS, copied with each of their four stages (the same bytes
+    // over themselves).  No branches around here: the compiler would move matrix instructions across them
+    auto copy = [&](int k, int buf, int i) {
+        if (i < S::LOADS) {
+            const uint8_t *base = (i < S::LOADS_A ? a0 : b0) + (int64_t)k * F8_BLOCK;
             uint32_t o = off[i];
-            asm("" : "+v"(o));
-            f8_copy16(i < S::LOADS_A ? a : b, o, dst + i * S::WAVES * 8 * F8_BLOCK);
+            asm("" : "+s"(base), "+v"(o));              // scalar base and 32-bit offset: one register per copy and lane
+            f8_copy16(base, o, lds0 + buf * S::STAGE + (i * S::WAVES + wave) * 8 * F8_BLOCK);
+        } else {                                        // (an operand's scales are followed by 1 KB that may be read)
+            const uint32_t *base = s0 + (k >> 2) * s_rows;
+            asm("" : "+s"(base));
+            f8_copy4(base, lane * 4, lds0 + 2 * S::STAGE + ((k >> 2) & 1) * (S::ROWS * 4) + wave * 256);
         }
-        // (an operand's scales are followed by 1 KB that may be read)
-        const uint32_t *sc = s0 + (k >> 2) * s_rows;
-        asm("" : "+s"(sc));
-        f8_copy4(sc, lane * 4, lds0 + 2 * S::STAGE + ((k >> 2) & 1) * (S::ROWS * 4) + wave * 256);
     };
     // this lane's two pieces of a fragment (row lane % 16 of a tile, 32 codes of the block) and its scale, for the wave's
     // first tile of either operand; the other tiles lie at constant distances
@@ -321,8 +320,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__re
     f32x4 acc[NT][MT] = {};
     i32x8 fa[MT], fb;
     uint32_t ea[MT], eb;
-    copy(0, 0);
-    copy(nk > 1 ? 1 : 0, 1);
+    constexpr int HALF = S::LOADS / 2, EVERY = HALF < MT ? MT / HALF : 1;
+    static_assert(S::LOADS % 2 == 0 && HALF * EVERY == MT, "half a stage's copies in a column of tiles");
+#pragma unroll
+    for (int i = 0; i <= S::LOADS; ++i) copy(0, 0, i);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) copy(nk > 1 ? 1 : 0, 1, i);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -347,7 +350,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__re
                 eb = scale(sc_b, k, j + 1);
             } else {
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                copy(k + 2 < nk ? k + 2 : nk - 1, k & 1);
                 fb = frag(lo_b, hi_b, k + 1, 0);        // (behind the last stage: read and not used)
                 eb = scale(sc_b, k + 1, 0);
             }
@@ -365,7 +367,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__re
                 if (j + 1 == NT) {
                     fa[i] = frag(lo_a, hi_a, k + 1, i);
                     ea[i] = scale(sc_a, k + 1, i);
+                    if (i % EVERY == EVERY - 1) copy(k + 2 < nk ? k + 2 : nk - 1, k & 1, i / EVERY);
                     __builtin_amdgcn_sched_barrier(0);  // not earlier: the register is in use until here
+                }
+                if (j == 0) {
+                    if (i % EVERY == EVERY - 1) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, HALF + i / EVERY);
+                    if (i == MT - 1) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, S::LOADS);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
