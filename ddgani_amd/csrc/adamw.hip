@@ -22,9 +22,10 @@
 #define ADW_NT 256
 #define ADW_BLOCK DDG_ADAMW_BLOCK                 // elements that share a scale = one wave x 4 elements
 #define ADW_VEC 4
-#define ADW_UNITS 4                               // state blocks per wave
-#define ADW_CHUNK (ADW_NT * ADW_VEC * ADW_UNITS)  // elements per workgroup
+#define ADW_WIDE 4                                // state blocks per wave in the wide variant (1 in the other)
 #define ADW_TABLE 64
+#define ADW_FEW 1024                              // workgroups that sum all partial norms themselves, at most
+#define ADW_NORM_GRID 2048                        // workgroups of the norm per launch: eight per CU, 16 KB of partial sums
 #define ADW_TINY 7.888609052210118e-31f           // 2^-100: blocks below are stored as zeros (448 / max stays finite)
 
 struct AdwEntry {
@@ -35,81 +36,106 @@ struct AdwEntry {
     int32_t chunk0;                               // first workgroup
 };
 struct AdwTable {
-    AdwEntry t[ADW_TABLE];
+    AdwEntry t[ADW_TABLE];                        // behind `count`: chunk0 = INT32_MAX
     int count;
 };
+static_assert(ADW_TABLE == 64, "one lane looks at one entry");
 
+struct AdwScalars {
+    float step_size, root2;                       // lr / (1 - b1^t), sqrt(1 - b2^t)
+    uint32_t dither;                              // of the step
+};
 // device side of the handle (DDG_ADAMW_CONTROL_BYTES)
 struct AdwControl {
-    int64_t step;                                 // steps done, the current one included
-    float norm, clip;
-    float step_size, root2;                       // lr / (1 - b1^t), sqrt(1 - b2^t)
-    uint32_t dither;                              // of this step
+    int64_t step;                                 // steps done
+    float norm, clip;                             // of the last step
+    AdwScalars sc;
     int32_t skip;                                 // 1: the norm is not finite, nothing moves
+    int64_t next;                                 // step + 1, while a step without k_adamw_begin runs
+};
+struct AdwHyper {
+    double lr, b1, b2;
+    float max_norm;                               // <= 0: no clip
 };
 
-__device__ __forceinline__ int adw_find(const AdwTable &tb, int chunk) {      // the last tensor whose chunk0 <= chunk
-    int a = 0, b = tb.count;
-    while (b - a > 1) {
-        const int mid = (a + b) >> 1;
-        if (tb.t[mid].chunk0 <= chunk) a = mid; else b = mid;
-    }
-    return a;
+__device__ __forceinline__ double adw_power(double b, int64_t t) {
+    double r = 1.0;
+    for (; t; t >>= 1, b *= b)
+        if (t & 1) r *= b;
+    return r;
+}
+// bias corrections in fp64, as a host would form them
+__device__ __forceinline__ AdwScalars adw_scalars(const AdwHyper &h, int64_t t) {
+    return {(float)(h.lr / (1.0 - adw_power(h.b1, t))), (float)sqrt(1.0 - adw_power(h.b2, t)), (uint32_t)t * 2246822507u};
 }
 
-// one fp64 partial per workgroup; eight squares at a time are added in fp32, everything above in fp64
-template <class G> __global__ __launch_bounds__(ADW_NT) void k_adamw_sqsum(AdwTable tb, double *__restrict__ part) {
-    const AdwEntry &e = tb.t[adw_find(tb, blockIdx.x)];
-    const G *g = (const G *)e.g;
-    const int64_t base = (int64_t)(blockIdx.x - e.chunk0) * ADW_CHUNK;
+// the tensor of a workgroup: the last entry whose chunk0 <= chunk, one entry per lane
+__device__ __forceinline__ int adw_find(const AdwTable &tb, int chunk) {
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(tb.t[threadIdx.x & 63].chunk0 <= chunk)) - 1);
+}
+
+// the partial sums of squares -> norm and clip factor, in every thread of the workgroup; false: the norm is not finite
+template <int NT>
+__device__ __forceinline__ bool adw_clip(const double *__restrict__ part, int64_t parts, float max_norm, float &norm, float &clip) {
+    __shared__ double w[NT / 64];
     double sum = 0;
+    int64_t i = threadIdx.x;
+    for (; i + 3 * NT < parts; i += 4 * NT) sum += (part[i] + part[i + NT]) + (part[i + 2 * NT] + part[i + 3 * NT]);
+    for (; i < parts; i += NT) sum += part[i];
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int k = 0; k < NT / 64; ++k) sum += w[k];
+    norm = (float)sqrt(sum);
+    clip = max_norm / (norm + 1e-6f);
+    clip = clip < 1.f ? clip : 1.f;
+    return norm <= 3.402823466e38f;                              // false for NaN and infinity
+}
+
+// step number, scalars and (max_norm > 0) the clip factor of the step
+__global__ __launch_bounds__(1024) void k_adamw_begin(const double *__restrict__ part, int64_t parts, AdwHyper h, AdwControl *c) {
+    float norm, clip = 1.f;
+    bool ok = true;
+    if (h.max_norm > 0.f) ok = adw_clip<1024>(part, parts, h.max_norm, norm, clip);
+    if (threadIdx.x) return;
+    if (h.max_norm > 0.f) c->norm = norm;
+    c->skip = !ok;
+    if (!ok) return;
+    c->clip = clip;
+    c->sc = adw_scalars(h, ++c->step);
+}
+
+// One fp64 partial per workgroup, which takes every gridDim-th chunk; four or eight squares at a time are added in fp32,
+// everything above in fp64.  ctl (may be NULL): the first workgroup writes the number of the step that begins.
+template <class G, int UNITS>
+__global__ __launch_bounds__(ADW_NT) void k_adamw_sqsum(AdwTable tb, int chunks, double *__restrict__ part, AdwControl *ctl) {
+    constexpr int V = UNITS == 1 ? 4 : 8, LOADS = ADW_VEC * UNITS / V;
+    double sum = 0;
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const AdwEntry &e = tb.t[adw_find(tb, c)];
+        const int64_t base = (int64_t)(c - e.chunk0) * (ADW_NT * ADW_VEC * UNITS) + threadIdx.x * V;
+        float v[LOADS][V];
 #pragma unroll
-    for (int u = 0; u < ADW_CHUNK / (ADW_NT * 8); ++u) {
-        const int64_t i = base + (u * ADW_NT + threadIdx.x) * 8;
-        float v[8];
-        const int64_t left = e.n - i;
-        load_n<8>(g + i, left < 0 ? 0 : left > 8 ? 8 : (int)left, v);
-        float s = 0;
+        for (int u = 0; u < LOADS; ++u) {
+            const int64_t i = base + u * (ADW_NT * V), left = e.n - i;
+            load_n<V>((const G *)e.g + i, left < 0 ? 0 : left > V ? V : (int)left, v[u]);
+        }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += v[k] * v[k];
-        sum += s;
+        for (int u = 0; u < LOADS; ++u) {
+            float s = 0;
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += v[u][k] * v[u][k];
+            sum += s;
+        }
     }
     __shared__ double w[ADW_NT / 64];
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
-}
-
-// the step's scalars: norm and clip factor (max_norm > 0), step number, bias corrections in fp64 as the host would form them
-__global__ __launch_bounds__(1024) void k_adamw_begin(const double *__restrict__ part, int64_t parts, float max_norm, double lr,
-                                                      double b1, double b2, AdwControl *c) {
-    __shared__ double w[16];
-    double sum = 0;
-    for (int64_t i = threadIdx.x; i < parts; i += 1024) sum += part[i];
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
-    __syncthreads();
     if (threadIdx.x) return;
-    float clip = 1.f;
-    bool ok = true;
-    if (max_norm > 0.f) {
-        sum = 0;
-        for (int i = 0; i < 16; ++i) sum += w[i];
-        const float norm = (float)sqrt(sum);
-        ok = norm <= 3.402823466e38f;                            // false for NaN and infinity
-        clip = max_norm / (norm + 1e-6f);
-        clip = clip < 1.f ? clip : 1.f;
-        c->norm = norm;
-    }
-    c->skip = !ok;
-    if (!ok) return;
-    const int64_t t = c->step + 1;
-    c->step = t;
-    c->clip = clip;
-    c->step_size = (float)(lr / (1.0 - pow(b1, (double)t)));
-    c->root2 = (float)sqrt(1.0 - pow(b2, (double)t));
-    c->dither = (uint32_t)t * 2246822507u;
+    part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
+    if (ctl && blockIdx.x == 0) ctl->next = ctl->step + 1;
 }
 
 // maximum over the wave, in every lane
@@ -162,48 +188,85 @@ struct AdwState {
     float *ms, *vs, *master;
 };
 
-// A wave owns ADW_UNITS blocks of 256 elements, four consecutive elements per lane: every access is one contiguous piece
-// per wave, and a block's maximum is one reduction over the wave.  No contraction: the products round as the formulas read.
+// A wave owns UNITS blocks of 256 elements, four consecutive elements per lane: every access is one contiguous piece per
+// wave, and a block's maximum is one reduction over the wave.  All loads come first.  Workgroups take the table from its end:
+// what the norm read last is still in the 256 MB cache.  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
+// adds up the partial norms and forms the step's scalars itself, which is quicker than a launch of its own for them.
+// (One launch for norm and step, whose last workgroup to arrive goes on alone, is slower: an atomic that all XCDs share takes
+// 85 ns a workgroup.)
+// No contraction: the products round as the formulas read.
 #pragma clang fp contract(off)
-template <class P, class G, bool BITS8, bool MASTER>
-__global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, const AdwControl *__restrict__ ctl, float one_m_b1,
-                                                  float b2, float one_m_b2, float eps) {
-    if (ctl->skip) return;
-    const AdwEntry &e = tb.t[adw_find(tb, blockIdx.x)];
-    const float clip = ctl->clip, step_size = ctl->step_size, root2 = ctl->root2, keep = e.keep;
-    const uint32_t dither = ctl->dither;
-    P *p = (P *)e.p;
-    const G *g = (const G *)e.g;
+template <class P, class G, bool BITS8, bool MASTER, int UNITS, bool SELF>
+__global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, AdwControl *ctl, AdwHyper h, float one_m_b1, float b2,
+                                                  float one_m_b2, float eps, const double *__restrict__ part, int parts) {
+    const int chunk = (int)(gridDim.x - 1 - blockIdx.x);
+    const AdwEntry &e = tb.t[adw_find(tb, chunk)];
+    P *__restrict__ const p = (P *)e.p;
+    const G *__restrict__ const g = (const G *)e.g;
     const int lane = threadIdx.x & 63;
-    const int64_t base = (int64_t)(blockIdx.x - e.chunk0) * ADW_CHUNK + (threadIdx.x >> 6) * (ADW_UNITS * ADW_BLOCK);
+    const int64_t base = (int64_t)(chunk - e.chunk0) * (ADW_NT * ADW_VEC * UNITS) + (threadIdx.x >> 6) * (UNITS * ADW_BLOCK);
+    float gv[UNITS][ADW_VEC], wv[UNITS][ADW_VEC], mv[UNITS][ADW_VEC], vv[UNITS][ADW_VEC], ms[UNITS], vs[UNITS];
+    uint32_t mc[UNITS], vc[UNITS];
 #pragma unroll
-    for (int u = 0; u < ADW_UNITS; ++u) {
+    for (int u = 0; u < UNITS; ++u) {
+        const int64_t b = base + u * ADW_BLOCK, i = b + lane * ADW_VEC, f = e.off + i;
+        const int n = e.n - i >= ADW_VEC ? ADW_VEC : e.n > i ? (int)(e.n - i) : 0;
+        load_n<ADW_VEC>(g + i, n, gv[u]);
+        if (MASTER) load_n<ADW_VEC>(st.master + f, n, wv[u]);
+        else load_n<ADW_VEC>(p + i, n, wv[u]);
+        if (BITS8) {
+            mc[u] = load_codes((const uint8_t *)st.m + f, n);
+            vc[u] = load_codes((const uint8_t *)st.v + f, n);
+            const int64_t blk = (e.off + b) / ADW_BLOCK;
+            ms[u] = b < e.n ? st.ms[blk] : 0.f;
+            vs[u] = b < e.n ? st.vs[blk] : 0.f;
+        } else {
+            load_n<ADW_VEC>((const float *)st.m + f, n, mv[u]);
+            load_n<ADW_VEC>((const float *)st.v + f, n, vv[u]);
+        }
+    }
+    AdwScalars sc;
+    float clip;
+    if constexpr (SELF) {
+        float norm;
+        const int64_t t = ctl->next;
+        const bool ok = adw_clip<ADW_NT>(part, parts, h.max_norm, norm, clip);
+        if (chunk == 0 && threadIdx.x == 0) {
+            ctl->norm = norm;
+            if (ok) ctl->step = t;                                // (nobody reads it in this launch)
+        }
+        if (!ok) return;
+        sc = adw_scalars(h, t);
+    } else {
+        if (ctl->skip) return;
+        sc = ctl->sc;
+        clip = h.max_norm > 0.f ? ctl->clip : 1.f;
+    }
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
         const int64_t b = base + u * ADW_BLOCK;                   // first element of the block, of this lane's four: i
-        if (b >= e.n) return;
+        if (b >= e.n) break;
         const int64_t i = b + lane * ADW_VEC, f = e.off + i;
         const int n = e.n - i >= ADW_VEC ? ADW_VEC : e.n > i ? (int)(e.n - i) : 0;
-        float gv[ADW_VEC], w[ADW_VEC], m[ADW_VEC], v[ADW_VEC], r[ADW_VEC];
-        load_n<ADW_VEC>(g + i, n, gv);
-        if (MASTER) load_n<ADW_VEC>(st.master + f, n, w);
-        else load_n<ADW_VEC>(p + i, n, w);
-        const int64_t blk = (e.off + b) / ADW_BLOCK;
+        float w[ADW_VEC], m[ADW_VEC], v[ADW_VEC], r[ADW_VEC];
         if (BITS8) {
-            decode(load_codes((const uint8_t *)st.m + f, n), st.ms[blk], m);
-            decode(load_codes((const uint8_t *)st.v + f, n), st.vs[blk], v);
+            decode(mc[u], ms[u], m);
+            decode(vc[u], vs[u], v);
 #pragma unroll
             for (int k = 0; k < ADW_VEC; ++k) v[k] = v[k] * v[k];
-        } else {
-            load_n<ADW_VEC>((const float *)st.m + f, n, m);
-            load_n<ADW_VEC>((const float *)st.v + f, n, v);
         }
         float top_m = 0.f, top_r = 0.f;
 #pragma unroll
         for (int k = 0; k < ADW_VEC; ++k) {
-            const float gg = gv[k] * clip;
+            if (!BITS8) {
+                m[k] = mv[u][k];
+                v[k] = vv[u][k];
+            }
+            const float gg = gv[u][k] * clip;
             m[k] = m[k] + one_m_b1 * (gg - m[k]);
             v[k] = v[k] * b2 + one_m_b2 * gg * gg;
             r[k] = sqrtf(v[k]);
-            w[k] = w[k] * keep - step_size * (m[k] / (r[k] / root2 + eps));
+            w[k] = wv[u][k] * e.keep - sc.step_size * (m[k] / (r[k] / sc.root2 + eps));
             if (k < n) {
                 top_m = fmaxf(top_m, fabsf(m[k]));
                 top_r = fmaxf(top_r, r[k]);
@@ -212,6 +275,7 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, cons
         if (MASTER) store_n<ADW_VEC>(st.master + f, n, w);
         store_n<ADW_VEC>(p + i, n, w);
         if (BITS8) {
+            const int64_t blk = (e.off + b) / ADW_BLOCK;
             top_m = wave_max(top_m);
             top_r = wave_max(top_r);
             const float im = top_m >= ADW_TINY ? (1.f / top_m) * 448.f : 0.f, ir = top_r >= ADW_TINY ? (1.f / top_r) * 448.f : 0.f;
@@ -221,7 +285,7 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, cons
                 r[k] = r[k] * ir;
             }
             store_codes((uint8_t *)st.m + f, n, encode_nearest(m));
-            store_codes((uint8_t *)st.v + f, n, encode_dithered(r, (uint32_t)f, dither));
+            store_codes((uint8_t *)st.v + f, n, encode_dithered(r, (uint32_t)f, sc.dither));
             if (lane == 0) {
                 st.ms[blk] = top_m >= ADW_TINY ? top_m * (1.f / 448.f) : 0.f;
                 st.vs[blk] = top_r >= ADW_TINY ? top_r * (1.f / 448.f) : 0.f;
@@ -234,7 +298,12 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, cons
 }
 #pragma clang fp contract(on)
 
-static inline int64_t adw_chunks(int64_t n) { return ceil_div64(n, ADW_CHUNK); }
+static inline int64_t adw_chunk(bool wide) { return ADW_NT * ADW_VEC * (wide ? ADW_WIDE : 1); }
+static int64_t adw_total(const ddg_adamw_tensor *t, int n_tensors, bool wide) {
+    int64_t total = 0;
+    for (int i = 0; i < n_tensors; ++i) total += t[i].numel > 0 ? ceil_div64(t[i].numel, adw_chunk(wide)) : 0;
+    return total;
+}
 
 static int adw_check(const ddg_adamw_tensor *t, int n_tensors, int64_t state_len) {
     if (n_tensors < 0 || (n_tensors > 0 && !t) || state_len < 0) return DDG_E_ARG;
@@ -243,25 +312,29 @@ static int adw_check(const ddg_adamw_tensor *t, int n_tensors, int64_t state_len
             t[i].offset > state_len - t[i].numel || !ddg_type_ok(t[i].param_type) || !ddg_type_ok(t[i].grad_type))
             return DDG_E_ARG;
         if (t[i].numel > 0 && (!t[i].param || !t[i].grad)) return DDG_E_ARG;
-        if (adw_chunks(t[i].numel) > 0x7FFFFFFF / ADW_TABLE) return DDG_E_UNSUPPORTED;
+        if (ceil_div64(t[i].numel, adw_chunk(true)) > 0x7FFFFFFF / ADW_TABLE) return DDG_E_UNSUPPORTED;
     }
     return DDG_OK;
 }
 
+// One block per wave and workgroups of 1 024 elements while that gives at most ADW_FEW of them (a million elements: latency
+// counts), else four blocks per wave
+static inline bool adw_wide(const ddg_adamw_tensor *t, int n_tensors) { return adw_total(t, n_tensors, false) > ADW_FEW; }
+
 extern "C" size_t ddg_adamw_workspace_bytes(const ddg_adamw_tensor *tensors, int n_tensors) {
     if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return 0;
-    int64_t parts = 0;
-    for (int i = 0; i < n_tensors; ++i) parts += tensors[i].numel > 0 ? adw_chunks(tensors[i].numel) : 0;
+    const int64_t parts = adw_total(tensors, n_tensors, adw_wide(tensors, n_tensors));
     return (size_t)(parts > 0 ? parts : 1) * sizeof(double);
 }
 
-// calls f(table, chunks) for groups of at most ADW_TABLE non-empty tensors that `take` accepts, in their order
+// calls f(table, workgroups) for groups of at most ADW_TABLE non-empty tensors that `take` accepts, in their order
 template <class Take, class F>
-static int adw_groups(const ddg_adamw_tensor *t, int n_tensors, double lr, const Take &take, const F &f) {
+static int adw_groups(const ddg_adamw_tensor *t, int n_tensors, bool wide, double lr, const Take &take, const F &f) {
     AdwTable tb;
     tb.count = 0;
     int64_t chunks = 0;
     auto flush = [&]() {
+        for (int i = tb.count; i < ADW_TABLE; ++i) tb.t[i].chunk0 = INT32_MAX;
         const int rc = tb.count ? f(tb, chunks) : (int)DDG_OK;
         tb.count = 0;
         chunks = 0;
@@ -271,7 +344,7 @@ static int adw_groups(const ddg_adamw_tensor *t, int n_tensors, double lr, const
         if (t[i].numel == 0 || !take(t[i])) continue;
         tb.t[tb.count++] = {t[i].param, t[i].grad, t[i].numel, t[i].offset, (float)(1.0 - lr * (double)t[i].weight_decay),
                             (int32_t)chunks};
-        chunks += adw_chunks(t[i].numel);
+        chunks += ceil_div64(t[i].numel, adw_chunk(wide));
         if (tb.count == ADW_TABLE) {
             const int rc = flush();
             if (rc) return rc;
@@ -293,48 +366,74 @@ extern "C" int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, in
     if (((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq | (uintptr_t)control | (uintptr_t)workspace) & 7) return DDG_E_ARG;
     const hipStream_t s = (hipStream_t)stream;
     AdwControl *ctl = (AdwControl *)control;
+    static_assert(sizeof(AdwControl) <= DDG_ADAMW_CONTROL_BYTES, "control block");
     double *part = (double *)workspace;
+    const AdwHyper h = {lr, beta1, beta2, (float)max_norm};
+    const bool wide = adw_wide(tensors, n_tensors), clip = max_norm > 0;
+    const int64_t total = adw_total(tensors, n_tensors, wide);
+    const bool self = clip && !wide && total > 0;       // no k_adamw_begin
     int64_t parts = 0;
-    if (max_norm > 0) {
+    uint32_t types = 0;                                 // the (parameter, gradient) types that occur
+    for (int i = 0; i < n_tensors; ++i)
+        if (tensors[i].numel > 0) types |= 1u << (tensors[i].param_type * 3 + tensors[i].grad_type);
+    if (clip) {
         if (!workspace || workspace_bytes < ddg_adamw_workspace_bytes(tensors, n_tensors)) return DDG_E_WORKSPACE;
         for (int gt = DDG_F32; gt <= DDG_F16; ++gt) {
+            if (!(types & (0x49u << gt))) continue;
             const int r = adw_groups(
-                tensors, n_tensors, lr, [&](const ddg_adamw_tensor &t) { return t.grad_type == gt; },
+                tensors, n_tensors, wide, lr, [&](const ddg_adamw_tensor &t) { return t.grad_type == gt; },
                 [&](const AdwTable &tb, int64_t chunks) {
                     return ddg_with_type(gt, [&](auto g) {
-                        k_adamw_sqsum<decltype(g)><<<(unsigned)chunks, ADW_NT, 0, s>>>(tb, part + parts);
+                        using G = decltype(g);
+                        const int64_t grid = chunks < ADW_NORM_GRID ? chunks : ADW_NORM_GRID;
+                        if (wide) k_adamw_sqsum<G, ADW_WIDE><<<(unsigned)grid, ADW_NT, 0, s>>>(tb, (int)chunks, part + parts, nullptr);
+                        else k_adamw_sqsum<G, 1><<<(unsigned)grid, ADW_NT, 0, s>>>(tb, (int)chunks, part + parts, parts == 0 ? ctl : nullptr);
                         DDG_CHECK_LAUNCH();
-                        parts += chunks;
+                        parts += grid;
                         return (int)DDG_OK;
                     });
                 });
             if (r) return r;
         }
     }
-    k_adamw_begin<<<1, 1024, 0, s>>>(part, parts, (float)max_norm, lr, beta1, beta2, ctl);
-    DDG_CHECK_LAUNCH();
+    if (!self) {
+        k_adamw_begin<<<1, clip ? 1024 : 64, 0, s>>>(part, parts, h, ctl);
+        DDG_CHECK_LAUNCH();
+    }
     const AdwState st = {exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, masters};
     for (int pt = DDG_F32; pt <= DDG_F16; ++pt)
         for (int gt = DDG_F32; gt <= DDG_F16; ++gt) {
+            if (!(types >> (pt * 3 + gt) & 1)) continue;
+            // (chunk 0 of every group writes the step's number and norm: the same values)
             const int r = adw_groups(
-                tensors, n_tensors, lr, [&](const ddg_adamw_tensor &t) { return t.param_type == pt && t.grad_type == gt; },
+                tensors, n_tensors, wide, lr,
+                [&](const ddg_adamw_tensor &t) { return t.param_type == pt && t.grad_type == gt; },
                 [&](const AdwTable &tb, int64_t chunks) {
                     return ddg_with_type(pt, [&](auto p) {
                         return ddg_with_type(gt, [&](auto g) {
                             using P = decltype(p);
                             using G = decltype(g);
-                            auto go = [&](auto bits8, auto master) {
-                                k_adamw<P, G, decltype(bits8)::value, decltype(master)::value><<<(unsigned)chunks, ADW_NT, 0, s>>>(
-                                    tb, st, ctl, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps);
+                            auto go = [&](auto bits8, auto master, auto units, auto fin) {
+                                k_adamw<P, G, decltype(bits8)::value, decltype(master)::value, decltype(units)::value,
+                                        decltype(fin)::value><<<(unsigned)chunks, ADW_NT, 0, s>>>(
+                                    tb, st, ctl, h, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, part,
+                                    (int)parts);
                             };
                             const std::true_type yes;
                             const std::false_type no;
+                            const std::integral_constant<int, 1> one;
+                            const std::integral_constant<int, ADW_WIDE> more;
+                            auto size = [&](auto bits8, auto master) {
+                                if (wide) go(bits8, master, more, no);
+                                else if (self) go(bits8, master, one, yes);
+                                else go(bits8, master, one, no);
+                            };
                             if constexpr (sizeof(P) == 2) {           // (an fp32 parameter is its own master)
-                                if (masters && state_bits == 8) go(yes, yes);
-                                else if (masters) go(no, yes);
+                                if (masters && state_bits == 8) size(yes, yes);
+                                else if (masters) size(no, yes);
                             }
                             if (sizeof(P) == 4 || !masters) {
-                                if (state_bits == 8) go(yes, no); else go(no, no);
+                                if (state_bits == 8) size(yes, no); else size(no, no);
                             }
                             DDG_CHECK_LAUNCH();
                             return (int)DDG_OK;

@@ -6,6 +6,7 @@ pointers of contiguous tensors to libddgani_hip.so on torch's current HIP stream
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional, Sequence
 
@@ -698,52 +699,50 @@ def _type(t: torch.Tensor, what: str) -> int:
 
 def _matrix(t: torch.Tensor, what: str):
     """(pointer, elements between rows) of a 2-D device tensor whose rows are contiguous and do not overlap"""
-    if not t.is_cuda:
+    if t.get_device() < 0:
         raise _lib.DdgError("ddgani_amd ops need tensors on the GPU (no CPU fallback)")
     if t.dim() != 2:
         raise _lib.DdgError(f"{what}: expected a matrix, got {t.dim()} dimensions")
     rows, cols = t.shape
-    ld = t.stride(0) if rows > 1 else max(t.stride(0), cols)
-    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+    ld, inner = t.stride()
+    if rows <= 1 and ld < cols:
+        ld = cols
+    if (inner != 1 and cols > 1) or ld < cols:
         raise _lib.DdgError(f"{what}: rows must be contiguous")
     return t.data_ptr(), ld
 
 
-def _same_device(dev: torch.device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise _lib.DdgError(f"{name}: on {t.device}, expected {dev}")
+def _on(dev: int, *tensors):
+    """the current stream of device ``dev``, on which all tensors have to be"""
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise _lib.DdgError(f"tensors on different devices: {t.device} and cuda:{dev}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-class _On:
-    """makes a tensor's device current around a call, so that the work goes to that device's current stream"""
-
-    def __init__(self, dev: torch.device):
-        self.dev = dev
-        self.guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.dev.index:
-            self.guard = torch.cuda.device(self.dev)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(dev: int, fn, what: str, *args):
+    """fn(*args) with ``dev`` current, so that kernels go to the device of their stream"""
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc:
+        check(rc, what)
 
 
-def _scratch(nbytes: int, dev: torch.device):
-    """(tensor, pointer) of a call's own workspace.  From torch's allocator and not from the per-device cache: two streams,
-    and two captured graphs, get different memory."""
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    return ws, ws.data_ptr() if nbytes else None
+# workspaces of these operators come from torch's allocator at each call and not from the per-device cache above: two streams,
+# and two captured graphs, get different memory
+@functools.lru_cache(maxsize=256)
+def _bytes(name: str, *sizes: int) -> int:
+    return getattr(lib(), name)(*sizes)
 
 
 # ----------------------------------------------------------------------------- embedding
 def _ids(ids: torch.Tensor):
-    if ids.dtype not in (torch.int32, torch.int64):
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise _lib.DdgError(f"ids: expected int32 or int64, got {ids.dtype}")
-    return _ptr(ids), int(ids.dtype == torch.int64)
+    return _ptr(ids), int(ids.dtype is torch.int64)
 
 
 def embedding(ids, table, scale: float = 1.0, out_dtype: Optional[torch.dtype] = None, out=None):
@@ -756,14 +755,16 @@ def embedding(ids, table, scale: float = 1.0, out_dtype: Optional[torch.dtype] =
     if V < 1 or D < 1:
         raise _lib.DdgError("embedding: empty table")
     if out is None:
-        out = torch.empty((*ids.shape, D), dtype=out_dtype or table.dtype, device=table.device)
-    elif (out_dtype is not None and out.dtype != out_dtype) or (out.shape != (*ids.shape, D) and out.shape != (ids.numel(), D)):
-        raise _lib.DdgError("embedding: out has another shape or type")
-    op, ldo = (_ptr(out), D) if out.dim() != 2 else _matrix(out, "out")
-    _same_device(table.device, ids=ids, out=out)
-    with _On(table.device):
-        check(lib().ddg_embedding(ip, i64, ids.numel(), tp, _type(table, "table"), V, D, ld, float(scale), op,
-                                  _type(out, "out"), ldo, _stream()), "ddg_embedding")
+        out = table.new_empty((*ids.shape, D), dtype=out_dtype)
+        op, ldo = out.data_ptr(), D
+    else:
+        if (out_dtype is not None and out.dtype != out_dtype) or (out.shape != (*ids.shape, D) and out.shape != (ids.numel(), D)):
+            raise _lib.DdgError("embedding: out has another shape or type")
+        op, ldo = (_ptr(out), D) if out.dim() != 2 else _matrix(out, "out")
+    dev = table.get_device()
+    stream = _on(dev, ids, out)
+    _call(dev, lib().ddg_embedding, "ddg_embedding", ip, i64, ids.numel(), tp, _type(table, "table"), V, D, ld, float(scale), op,
+          _type(out, "out"), ldo, stream)
     return out
 
 
@@ -778,24 +779,20 @@ def embedding_grad(ids, dy, n_rows: int, scale: float = 1.0, padding_idx: Option
         raise _lib.DdgError(f"embedding_grad: dy {tuple(dy.shape)} does not match ids {tuple(ids.shape)}")
     if n_rows < 1 or D < 1:
         raise _lib.DdgError("embedding_grad: empty table")
-    if dy.dim() == 2:
-        dp, ld = _matrix(dy, "dy")
-    else:
-        dp, ld = _ptr(dy), D
+    dp, ld = (_ptr(dy), D) if dy.dim() != 2 else _matrix(dy, "dy")
     if out is None:
         if accumulate:
             raise _lib.DdgError("embedding_grad: accumulate needs out")
-        out = torch.empty((n_rows, D), dtype=out_dtype, device=dy.device)
+        out = dy.new_empty((n_rows, D), dtype=out_dtype)
     elif out.shape != (n_rows, D):
         raise _lib.DdgError(f"embedding_grad: out {tuple(out.shape)}, expected {(n_rows, D)}")
     op, ldo = _matrix(out, "out")
-    _same_device(dy.device, ids=ids, out=out)
-    with _On(dy.device):
-        nb = lib().ddg_embedding_grad_workspace_bytes(n, D)
-        ws, wp = _scratch(nb, dy.device)
-        check(lib().ddg_embedding_grad(ip, i64, n, dp, _type(dy, "dy"), ld, int(n_rows), D, float(scale),
-                                       -1 if padding_idx is None else int(padding_idx), int(accumulate), op, _type(out, "out"),
-                                       ldo, wp, nb, _stream()), "ddg_embedding_grad")
+    dev = dy.get_device()
+    stream = _on(dev, ids, out)
+    nb = _bytes("ddg_embedding_grad_workspace_bytes", n, D)
+    ws = dy.new_empty(nb, dtype=torch.uint8)
+    _call(dev, lib().ddg_embedding_grad, "ddg_embedding_grad", ip, i64, n, dp, _type(dy, "dy"), ld, int(n_rows), D,
+          float(scale), -1 if padding_idx is None else int(padding_idx), bool(accumulate), op, _type(out, "out"), ldo, ws.data_ptr(), nb, stream)
     return out
 
 
@@ -809,8 +806,7 @@ class Fp8Weight:
         self.out_dim, self.in_dim = W.shape
         if self.out_dim < 1 or self.in_dim < 1:
             raise _lib.DdgError("Fp8Weight: empty weight")
-        self.device = W.device
-        buf = lambda r, c: torch.empty(lib().ddg_fp8_operand_bytes(r, c), dtype=torch.uint8, device=W.device)
+        buf = lambda r, c: W.new_empty(lib().ddg_fp8_operand_bytes(r, c), dtype=torch.uint8)
         self.packed = buf(self.out_dim, self.in_dim)
         self.packed_t = buf(self.in_dim, self.out_dim) if grads else None
         self.refresh(W)
@@ -819,10 +815,10 @@ class Fp8Weight:
         if tuple(W.shape) != (self.out_dim, self.in_dim):
             raise _lib.DdgError(f"Fp8Weight: expected {(self.out_dim, self.in_dim)}, got {tuple(W.shape)}")
         wp, ld = _matrix(W, "W")
-        _same_device(self.device, W=W)
-        with _On(self.device):
-            check(lib().ddg_fp8_pack_weight(wp, _type(W, "W"), ld, self.out_dim, self.in_dim, self.packed.data_ptr(),
-                                            _ptr(self.packed_t), _stream()), "ddg_fp8_pack_weight")
+        dev = W.get_device()
+        stream = _on(dev, self.packed)
+        _call(dev, lib().ddg_fp8_pack_weight, "ddg_fp8_pack_weight", wp, _type(W, "W"), ld, self.out_dim, self.in_dim,
+              self.packed.data_ptr(), _ptr(self.packed_t), stream)
 
 
 def linear_fp8(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype] = None, out=None):
@@ -830,21 +826,24 @@ def linear_fp8(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype]
     x is quantised within the call, in groups of 128 along its rows; up to 16 rows take one launch."""
     xp, ld = _matrix(x, "x")
     rows, inn = x.shape
+    outd = weight.out_dim
     if inn != weight.in_dim:
         raise _lib.DdgError(f"linear_fp8: x has {inn} columns, the weight {weight.in_dim}")
-    if bias is not None and bias.shape != (weight.out_dim,):
+    if bias is not None and bias.shape != (outd,):
         raise _lib.DdgError("linear_fp8: bias has another length than the layer's output")
     if out is None:
-        out = torch.empty((rows, weight.out_dim), dtype=out_dtype or x.dtype, device=x.device)
-    elif out.shape != (rows, weight.out_dim) or (out_dtype is not None and out.dtype != out_dtype):
-        raise _lib.DdgError("linear_fp8: out has another shape or type")
-    op, ldo = _matrix(out, "out")
-    _same_device(x.device, weight=weight.packed, bias=bias, out=out)
-    with _On(x.device):
-        nb = lib().ddg_fp8_linear_workspace_bytes(rows, inn)
-        ws, wp = _scratch(nb, x.device)
-        check(lib().ddg_fp8_linear(xp, _type(x, "x"), ld, rows, weight.packed.data_ptr(), weight.out_dim, inn,
-                                   _ptr(bias, torch.float32), op, _type(out, "out"), ldo, wp, nb, _stream()), "ddg_fp8_linear")
+        out = x.new_empty((rows, outd), dtype=out_dtype)
+        op, ldo = out.data_ptr(), outd
+    else:
+        if out.shape != (rows, outd) or (out_dtype is not None and out.dtype != out_dtype):
+            raise _lib.DdgError("linear_fp8: out has another shape or type")
+        op, ldo = _matrix(out, "out")
+    dev = x.get_device()
+    stream = _on(dev, weight.packed, bias, out)
+    nb = _bytes("ddg_fp8_linear_workspace_bytes", rows, inn)
+    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
+    _call(dev, lib().ddg_fp8_linear, "ddg_fp8_linear", xp, _type(x, "x"), ld, rows, weight.packed.data_ptr(), outd, inn,
+          _ptr(bias, torch.float32), op, _type(out, "out"), ldo, ws.data_ptr() if nb else None, nb, stream)
     return out
 
 
@@ -854,27 +853,25 @@ def linear_fp8_grads(dy, x, weight: Fp8Weight, want_bias: bool = False, out_dtyp
     dp, ldd = _matrix(dy, "dy")
     xp, ldx = _matrix(x, "x")
     rows, inn = x.shape
-    if inn != weight.in_dim or dy.shape != (rows, weight.out_dim):
-        raise _lib.DdgError(f"linear_fp8_grads: dy {tuple(dy.shape)}, x {tuple(x.shape)}, weight {(weight.out_dim, inn)}")
+    outd = weight.out_dim
+    if inn != weight.in_dim or dy.shape != (rows, outd):
+        raise _lib.DdgError(f"linear_fp8_grads: dy {tuple(dy.shape)}, x {tuple(x.shape)}, weight {(outd, inn)}")
     if weight.packed_t is None:
         raise _lib.DdgError("linear_fp8_grads: the weight was packed with grads=False")
-    dev, out_dim = x.device, weight.out_dim
-    _same_device(dev, dy=dy, weight=weight.packed)
-    code = _TYPE.get(out_dtype or dy.dtype)
-    if code is None:
-        raise _lib.DdgError("linear_fp8_grads: dx in float32, bfloat16 or float16")
-    new = torch.zeros if rows == 0 else torch.empty             # no rows: no products, the sums over them are zero
-    dx = torch.empty((rows, inn), dtype=out_dtype or dy.dtype, device=dev)
-    dw = new((out_dim, inn), dtype=torch.float32, device=dev)
-    db = new((out_dim,), dtype=torch.float32, device=dev) if want_bias else None
+    dev = x.get_device()
+    stream = _on(dev, dy, weight.packed)
+    new = x.new_empty if rows else x.new_zeros                  # no rows: no products, the sums over them are zero
+    dx = dy.new_empty((rows, inn), dtype=out_dtype)
+    dw = new((outd, inn), dtype=torch.float32)
+    db = new((outd,), dtype=torch.float32) if want_bias else None
+    dxt = _type(dx, "dx")
     if rows == 0:
         return dx, dw, db
-    with _On(dev):
-        nb = lib().ddg_fp8_linear_grads_workspace_bytes(rows, out_dim, inn)
-        ws, wp = _scratch(nb, dev)
-        check(lib().ddg_fp8_linear_grads(dp, _type(dy, "dy"), ldd, xp, _type(x, "x"), ldx, rows, weight.packed_t.data_ptr(),
-                                         out_dim, inn, dx.data_ptr(), code, inn, dw.data_ptr(), _ptr(db), wp, nb, _stream()),
-              "ddg_fp8_linear_grads")
+    nb = _bytes("ddg_fp8_linear_grads_workspace_bytes", rows, outd, inn)
+    ws = x.new_empty(nb, dtype=torch.uint8)
+    _call(dev, lib().ddg_fp8_linear_grads, "ddg_fp8_linear_grads", dp, _type(dy, "dy"), ldd, xp, _type(x, "x"), ldx, rows,
+          weight.packed_t.data_ptr(), outd, inn, dx.data_ptr(), dxt, inn, dw.data_ptr(), None if db is None else db.data_ptr(),
+          ws.data_ptr(), nb, stream)
     return dx, dw, db
 
 
@@ -924,7 +921,8 @@ class AdamW:
         zeros = lambda n, dt: torch.zeros(n, dtype=dt, device=dev)
         code = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
         _type_of = [_type(p, "params") for p in self.params]
-        _same_device(dev, **{f"params[{i}]": p for i, p in enumerate(self.params)})
+        self.dev = dev.index
+        _on(self.dev, *self.params)
         # (zeros as bytes: a fill kernel is not needed for every element type)
         self.exp_avg = zeros(total * code.itemsize, torch.uint8).view(code)
         self.exp_avg_sq = zeros(total * code.itemsize, torch.uint8).view(code)
@@ -940,6 +938,8 @@ class AdamW:
         self._t = (_lib.AdamwTensor * len(self.params))()
         for i, p in enumerate(self.params):
             self._t[i] = _lib.AdamwTensor(_ptr(p), None, p.numel(), self.offsets[i], self.weight_decay[i], _type_of[i], 0, 0)
+        self._state = (self._t, len(self._t), state_bits, _ptr(self.exp_avg), _ptr(self.exp_avg_sq), _ptr(self.exp_avg_scale),
+                       _ptr(self.exp_avg_sq_scale), _ptr(self.masters), total)
         self._ws = None
         self.set_grads(grads)
 
@@ -952,7 +952,7 @@ class AdamW:
             if g.shape != p.shape:
                 raise _lib.DdgError(f"AdamW: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
         ptr = [(_ptr(g), _type(g, "grads")) for g in grads]
-        _same_device(self.device, **{f"grads[{i}]": g for i, g in enumerate(grads)})
+        _on(self.dev, *grads)
         for t, (p, code) in zip(self._t, ptr):
             t.grad, t.grad_type = p, code
         self.grads = grads
@@ -965,12 +965,9 @@ class AdamW:
         if lr is not None:
             self.lr = lr
         clip = self.max_norm is not None
-        with _On(self.device):
-            check(lib().ddg_adamw_step(self._t, len(self._t), self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                                       _ptr(self.exp_avg_scale), _ptr(self.exp_avg_sq_scale), _ptr(self.masters), self.state_len,
-                                       self.lr, self.betas[0], self.betas[1], self.eps, self.max_norm if clip else 0.0,
-                                       self.control.data_ptr(), _ptr(self._ws), self._ws.numel() if clip else 0, _stream()),
-                  "ddg_adamw_step")
+        _call(self.dev, lib().ddg_adamw_step, "ddg_adamw_step", *self._state, self.lr, *self.betas, self.eps,
+              self.max_norm if clip else 0.0, self.control.data_ptr(), self._ws.data_ptr() if clip else None,
+              self._ws.numel() if clip else 0, _on(self.dev))
         return self.norm if clip else None
 
     def state_dict(self):
