@@ -10,10 +10,46 @@
 // reproducible), and written once.  Frequent ids are long rows: sorted positions are cut into aligned chunks of 64, and a
 // chunk that belongs to ONE id is summed beforehand by k_embg_part (4 096-chunks of such sums by a second launch), so the
 // longest walk a row can need is 63 + 63 single tokens, 63 + 63 sums of 64 and n / 4 096 sums of 4 096.
+#include <type_traits>
 #include "types.h"
 
 #define EMB_NT 256
 #define EMB_VEC 8                     // elements per thread and row: 16 bytes of a 16-bit type
+
+// A lane's eight columns of rows of D: [at, at + 8) is what it loads, always whole and inside the row, so that no load sits
+// behind a branch and several stay in flight; `col` on is what it writes (the last lane's piece overlaps its neighbour's, a
+// lane behind the row repeats the last piece and writes nothing).  TINY: D < 8, one lane, element by element.
+struct Columns {
+    int col, at, D;
+    __device__ Columns(int c, int d) : col(c), at(c < d - EMB_VEC ? c : d > EMB_VEC ? d - EMB_VEC : 0), D(d) {}
+};
+template <class T> using vec8 = T __attribute__((ext_vector_type(EMB_VEC)));
+template <bool TINY, class T> __device__ __forceinline__ vec8<T> load_row(const T *row, const Columns &c) {
+    vec8<T> v;
+    if (TINY) {
+#pragma unroll
+        for (int i = 0; i < EMB_VEC; ++i) v[i] = i < c.D ? row[i] : (T)0.f;
+    } else {
+        __builtin_memcpy(&v, row + c.at, sizeof(v));
+    }
+    return v;
+}
+template <bool TINY, class T> __device__ __forceinline__ void store_row(T *row, const Columns &c, const float (&v)[EMB_VEC]) {
+    vec8<T> o;
+#pragma unroll
+    for (int i = 0; i < EMB_VEC; ++i) o[i] = (T)v[i];
+    if (!TINY && c.col == c.at) {
+        __builtin_memcpy(row + c.at, &o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int i = 0; i < EMB_VEC; ++i)
+            if (c.at + i >= c.col && c.at + i < c.D) row[c.at + i] = o[i];
+    }
+}
+template <class T> __device__ __forceinline__ void add_row(float (&acc)[EMB_VEC], const vec8<T> &v) {
+#pragma unroll
+    for (int i = 0; i < EMB_VEC; ++i) acc[i] += (float)v[i];
+}
 
 template <class ID> __device__ __forceinline__ uint32_t emb_key(const ID *ids, int64_t i, int64_t V, int64_t padding_idx) {
     const int64_t v = (int64_t)ids[i];
@@ -21,29 +57,27 @@ template <class ID> __device__ __forceinline__ uint32_t emb_key(const ID *ids, i
 }
 
 // U rows per thread group: their id loads, then their row loads, are in flight together
-template <class TI, class TO, class ID, int U>
+template <class TI, class TO, class ID, int U, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embed(const ID *__restrict__ ids, int64_t n, const TI *__restrict__ table, int64_t V,
                                                   int D, int64_t ld, float scale, TO *__restrict__ out, int64_t ldo, int lg_tpr) {
     const int tpr = 1 << lg_tpr, rpb = EMB_NT >> lg_tpr;
-    const int col = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * EMB_VEC;
+    const Columns c((blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * EMB_VEC, D);
     const int64_t row0 = (int64_t)blockIdx.x * (rpb * U) + (threadIdx.x >> lg_tpr);
-    if (col >= D) return;
+    if (c.col >= D) return;
     int64_t id[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) id[u] = row0 + (int64_t)u * rpb < n ? (int64_t)ids[row0 + (int64_t)u * rpb] : -1;
-    float v[U][EMB_VEC];
+    vec8<TI> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const bool ok = (uint64_t)id[u] < (uint64_t)V;
-        load_n<EMB_VEC>(table + (ok ? id[u] : 0) * ld + col, ok ? D - col : 0, v[u]);      // outside the table: zeros
-    }
+    for (int u = 0; u < U; ++u) v[u] = load_row<TINY>(table + ((uint64_t)id[u] < (uint64_t)V ? id[u] : 0) * ld, c);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t r = row0 + (int64_t)u * rpb;
         if (r >= n) return;
+        float f[EMB_VEC];
 #pragma unroll
-        for (int i = 0; i < EMB_VEC; ++i) v[u][i] *= scale;
-        store_n<EMB_VEC>(out + r * ldo + col, D - col, v[u]);
+        for (int i = 0; i < EMB_VEC; ++i) f[i] = (uint64_t)id[u] < (uint64_t)V ? (float)v[u][i] * scale : 0.f;
+        store_row<TINY>(out + r * ldo, c, f);
     }
 }
 
@@ -72,13 +106,15 @@ extern "C" int ddg_embedding(const void *ids, int ids_64, int64_t n, const void 
             using TO = decltype(to);
             auto go = [&](auto id) {
                 using ID = decltype(id);
-                const dim3 grid((unsigned)gx, (unsigned)slabs);
-                if (wide)
-                    k_embed<TI, TO, ID, 4><<<grid, EMB_NT, 0, (hipStream_t)stream>>>(
-                        (const ID *)ids, n, (const TI *)table, V, D, ld_table, scale, (TO *)out, ld_out, lg);
-                else
-                    k_embed<TI, TO, ID, 1><<<grid, EMB_NT, 0, (hipStream_t)stream>>>(
-                        (const ID *)ids, n, (const TI *)table, V, D, ld_table, scale, (TO *)out, ld_out, lg);
+                auto launch = [&](auto u, auto tiny) {
+                    k_embed<TI, TO, ID, decltype(u)::value, decltype(tiny)::value>
+                        <<<dim3((unsigned)gx, (unsigned)slabs), EMB_NT, 0, (hipStream_t)stream>>>(
+                            (const ID *)ids, n, (const TI *)table, V, D, ld_table, scale, (TO *)out, ld_out, lg);
+                };
+                const std::integral_constant<int, 4> four;
+                const std::integral_constant<int, 1> one;
+                if (D < EMB_VEC) wide ? launch(four, std::true_type()) : launch(one, std::true_type());
+                else wide ? launch(four, std::false_type()) : launch(one, std::false_type());
                 DDG_CHECK_LAUNCH();
                 return (int)DDG_OK;
             };
@@ -197,10 +233,15 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_scatter(SortSrc<ID> src, int64
     for (int64_t i = slo + (t & 63); i < shi; i += 64) atomicAdd(&next[w][(src.k(i) >> shift) & (bins - 1)], 1u);
     uint32_t before = 0, total = 0;
     if (t < bins)
-        for (int b = 0; b < tiles; ++b) {
-            const uint32_t h = hist[(int64_t)b * SORT_BINS + t];
-            total += h;
-            if (b < (int)blockIdx.x) before += h;
+        for (int b = 0; b < tiles; b += 16) {           // (sixteen loads in flight: a loop of single ones took 30 us)
+            uint32_t h[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) h[u] = b + u < tiles ? hist[(int64_t)(b + u) * SORT_BINS + t] : 0;
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                total += h[u];
+                if (b + u < (int)blockIdx.x) before += h[u];
+            }
         }
     __syncthreads();
     uint32_t at = block_exclusive(total, wsum) + before;
@@ -263,98 +304,172 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_sort_small(const ID *__restric
 // ---------------------------------------------------------------------------------------------
 // sums
 // ---------------------------------------------------------------------------------------------
-// acc += rows src[index(j)] (columns from col on) for j in [a, b), four rows in flight
-template <class T, class Idx>
-__device__ __forceinline__ void add_rows(const T *__restrict__ src, int64_t ld, int col, int D, int64_t a, int64_t b,
-                                         const Idx &index, float (&acc)[EMB_VEC]) {
-    float v[4][EMB_VEC];
+// acc += rows [a, b) of src, four rows in flight
+template <bool TINY>
+__device__ __forceinline__ void add_rows(const float *__restrict__ src, const Columns &c, uint32_t a, uint32_t b,
+                                         float (&acc)[EMB_VEC]) {
+    vec8<float> v[4];
     for (; a + 4 <= b; a += 4) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_n<EMB_VEC>(src + (int64_t)index(a + u) * ld + col, D - col, v[u]);
+        for (int u = 0; u < 4; ++u) v[u] = load_row<TINY>(src + (int64_t)(a + u) * c.D, c);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int i = 0; i < EMB_VEC; ++i) acc[i] += v[u][i];
+        for (int u = 0; u < 4; ++u) add_row<float>(acc, v[u]);
     }
-    for (; a < b; ++a) {
-        load_n<EMB_VEC>(src + (int64_t)index(a) * ld + col, D - col, v[0]);
-#pragma unroll
-        for (int i = 0; i < EMB_VEC; ++i) acc[i] += v[0][i];
-    }
+    for (; a < b; ++a) add_row<float>(acc, load_row<TINY>(src + (int64_t)a * c.D, c));
 }
 
 // LEVEL 1: part[c] = sum of the dy rows of sorted positions [64 c, 64 c + 64) if they all belong to one row of the table;
 // LEVEL 2: part[c] = sum of the LEVEL-1 sums of [4 096 c, ...), under the same condition.  Other chunks are never read.
-template <class T, int LEVEL>
+template <class T, int LEVEL, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
                                                       int64_t chunks, uint32_t V, const T *__restrict__ src, int64_t ld, int D,
                                                       float *__restrict__ part, int lg_tpr) {
     const int tpr = 1 << lg_tpr;
-    const int col = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * EMB_VEC;
+    const Columns cs((blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * EMB_VEC, D);
     const int64_t c = (int64_t)blockIdx.x * (EMB_NT >> lg_tpr) + (threadIdx.x >> lg_tpr);
     const int len = LEVEL == 1 ? CHUNK1 : CHUNK2;
-    if (c >= chunks || col >= D) return;
+    if (c >= chunks || cs.col >= D) return;
     const uint32_t k = key[c * len];
     if (k >= V || k != key[c * len + len - 1]) return;
     float acc[EMB_VEC] = {};
-    if (LEVEL == 1)
-        add_rows(src, ld, col, D, c * CHUNK1, (c + 1) * CHUNK1, [&](int64_t j) { return pos[j]; }, acc);
-    else
-        add_rows(src, ld, col, D, c * (CHUNK2 / CHUNK1), (c + 1) * (CHUNK2 / CHUNK1), [](int64_t j) { return j; }, acc);
-    store_n<EMB_VEC>(part + c * D + col, D - col, acc);
+    uint32_t p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * 64 + u] : (uint32_t)(c * 64 + u);
+    for (int j = 0; j < 64; j += 8) {                   // eight rows in flight, and with them the next eight positions
+        vec8<T> v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = load_row<TINY>(src + (int64_t)p[u] * ld, cs);
+        const int next = j + 8 < 64 ? j + 8 : j;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * 64 + next + u] : (uint32_t)(c * 64 + next + u);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) add_row<T>(acc, v[u]);
+    }
+    store_row<TINY>(part + c * D, cs, acc);
 }
 
-#define ROWS_MAX 32                   // table rows per workgroup of k_embg_rows
+// How the sorted positions [a, b) of a row divide: single tokens [a, a1) and [b1, b), sums of 64 [a1, a2) and [b2, b1), sums
+// of 4 096 [a2, b2)
+struct RowParts {
+    uint32_t a, a1, a2, b2, b1, b;
+};
+__device__ __forceinline__ RowParts row_parts(uint32_t a, uint32_t b) {
+    RowParts p = {a, b, b, b, b, b};
+    const uint32_t up1 = (a + CHUNK1 - 1) / CHUNK1 * CHUNK1, dn1 = b / CHUNK1 * CHUNK1;
+    if (up1 >= dn1) return p;                           // no whole chunk
+    p.a1 = up1;
+    p.b1 = dn1;
+    const uint32_t up2 = (a + CHUNK2 - 1) / CHUNK2 * CHUNK2, dn2 = b / CHUNK2 * CHUNK2;
+    p.a2 = up2 < dn2 ? up2 : dn1;
+    p.b2 = up2 < dn2 ? dn2 : dn1;
+    return p;
+}
 
-template <class T, class TO>
+#define ROWS_MAX 32                   // table rows per wave, at most: one lane finds the positions of one row
+
+// A group of 2^lg lanes owns `rows` consecutive rows of the table and as many columns as it has lanes x 8.  The single tokens
+// of all its rows form one list, which is walked four at a time with the next four loads in flight, across the rows' borders:
+// most rows have few tokens, and a walk row by row would wait out the memory's latency for each of them (609 us, now
+// ROWS_US, for 262 144 tokens of 2 048 elements in 128 000 rows).
+template <class T, class TO, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n,
                                                       int64_t V, const T *__restrict__ dy, int64_t ld, int D,
                                                       const float *__restrict__ part1, const float *__restrict__ part2, float scale,
-                                                      int accumulate, TO *__restrict__ out, int64_t ldo, int lg_tpr, int rows) {
-    __shared__ int64_t start[ROWS_MAX + 1];
-    const int64_t v0 = (int64_t)blockIdx.x * rows;
-    if (threadIdx.x <= rows) {                          // first sorted position whose key is >= v
-        const uint64_t v = v0 + threadIdx.x;
-        int64_t a = 0, b = n;
-        while (a < b) {
-            const int64_t mid = (a + b) >> 1;
-            if (key[mid] < v) a = mid + 1; else b = mid;
+                                                      int accumulate, TO *__restrict__ out, int64_t ldo, int lg, int rows) {
+    const int lane = threadIdx.x & 63, lanes = 1 << lg, in_group = lane & (lanes - 1), group = lane >> lg;
+    const int64_t wave0 = ((int64_t)blockIdx.x * (EMB_NT / 64) + (threadIdx.x >> 6)) * ((64 >> lg) * rows);
+    if (wave0 >= V) return;
+    // lane l: the first sorted position whose key is >= row wave0 + l
+    int64_t lo = 0, hi = n;
+    {
+        const uint64_t v = wave0 + lane;
+        while (__any(lo < hi)) {
+            const int64_t mid = (lo + hi) >> 1;
+            const bool go = lo < hi, less = go && key[mid] < v;
+            if (go && less) lo = mid + 1;
+            if (go && !less) hi = mid;
         }
-        start[threadIdx.x] = a;
     }
-    __syncthreads();
-    const int tpr = 1 << lg_tpr;
-    const int col = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * EMB_VEC;
-    if (col >= D) return;
-    for (int r = threadIdx.x >> lg_tpr; r < rows && v0 + r < V; r += EMB_NT >> lg_tpr) {
-        int64_t a = start[r];
-        const int64_t b = start[r + 1];
-        if (accumulate && a == b) continue;
-        float acc[EMB_VEC] = {};
-        while (a < b) {                                 // the longest whole chunk that starts here, else single tokens
-            if (a % CHUNK2 == 0 && a + CHUNK2 <= b) {
-                const int64_t m = (b - a) / CHUNK2;
-                add_rows(part2, D, col, D, a / CHUNK2, a / CHUNK2 + m, [](int64_t j) { return j; }, acc);
-                a += m * CHUNK2;
-            } else if (a % CHUNK1 == 0 && a + CHUNK1 <= b) {
-                int64_t m = (b - a) / CHUNK1;           // up to the next multiple of CHUNK2 (a whole one is taken above)
-                const int64_t to2 = (CHUNK2 - a % CHUNK2) / CHUNK1;
-                if (m > to2) m = to2;
-                add_rows(part1, D, col, D, a / CHUNK1, a / CHUNK1 + m, [](int64_t j) { return j; }, acc);
-                a += m * CHUNK1;
-            } else {
-                const int64_t next1 = (a / CHUNK1 + 1) * CHUNK1, e = next1 < b ? next1 : b;
-                add_rows(dy, ld, col, D, a, e, [&](int64_t j) { return pos[j]; }, acc);
-                a = e;
+    const Columns c((blockIdx.y * lanes + in_group) * EMB_VEC, D);
+    const int64_t v0 = wave0 + group * rows;
+    // lane r of the group: row r's positions and single tokens, and how many the rows up to it have.  From here on groups go
+    // their own ways and exchange data within themselves only
+    const int own = group * rows + (in_group < rows ? in_group : rows - 1);
+    const int first = __shfl((int)lo, own), behind = __shfl((int)lo, own + 1);
+    const RowParts rp = row_parts(first, behind);
+    const int singles = in_group < rows && v0 + in_group < V ? (int)(rp.a1 - rp.a + rp.b - rp.b1) : 0;
+    int upto = singles;                                 // inclusive prefix over the group's rows
+    for (int d = 1; d < lanes; d <<= 1) {
+        const int y = __shfl_up(upto, d, lanes);
+        if (in_group >= d) upto += y;
+    }
+    const int total = __shfl(upto, lanes - 1, lanes);
+
+    float acc[EMB_VEC] = {};
+    int row = 0;                                        // row of the group whose sum acc is
+    auto finish = [&]() {                               // writes row `row`, begins the next
+        const int64_t v = v0 + row;
+        const uint32_t a = __shfl(first, row, lanes), b = __shfl(behind, row, lanes);
+        if (v < V && c.col < D && !(accumulate && a == b)) {
+            const RowParts p = row_parts(a, b);
+            if (p.a1 < p.b1) {
+                add_rows<TINY>(part1, c, p.a1 / CHUNK1, p.a2 / CHUNK1, acc);
+                add_rows<TINY>(part2, c, p.a2 / CHUNK2, p.b2 / CHUNK2, acc);
+                add_rows<TINY>(part1, c, p.b2 / CHUNK1, p.b1 / CHUNK1, acc);
+            }
+            TO *o = out + v * ldo;
+            vec8<TO> old = {};
+            if (accumulate) old = load_row<TINY>(o, c);
+#pragma unroll
+            for (int i = 0; i < EMB_VEC; ++i) acc[i] = (float)old[i] + scale * acc[i];
+            store_row<TINY>(o, c, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < EMB_VEC; ++i) acc[i] = 0.f;
+        ++row;
+    };
+
+    vec8<T> v[2][4];
+    int r[2][4];
+    int item_pos = 0, item_row = rows;                  // this lane's item of the current batch of `lanes` items
+    auto fetch = [&](int j, vec8<T>(&w)[4], int (&rr)[4]) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {                   // (behind the list: token 0, not used)
+            const int q = __shfl(item_pos, j + u, lanes);
+            rr[u] = __shfl(item_row, j + u, lanes);
+            w[u] = load_row<TINY>(dy + (int64_t)q * ld, c);
+        }
+    };
+    for (int base = 0; base < total; base += lanes) {
+        // lane l: item base + l of the list, its row by counting the rows that end before it
+        const int it = base + in_group;
+        int rr = 0;
+        for (int k = 0; k < rows; ++k) rr += __shfl(upto, k, lanes) <= it;
+        const int rc = rr < rows ? rr : rows - 1;
+        const uint32_t ordinal = it - (__shfl(upto, rc, lanes) - __shfl(singles, rc, lanes));
+        const RowParts p = row_parts(__shfl(first, rc, lanes), __shfl(behind, rc, lanes));
+        const uint32_t at = ordinal < p.a1 - p.a ? p.a + ordinal : p.b1 + (ordinal - (p.a1 - p.a));
+        item_row = it < total ? rr : rows;
+        item_pos = it < total ? (int)pos[at] : 0;
+        const int steps = total - base < lanes ? (total - base + 3) / 4 : (lanes + 3) / 4;
+        fetch(0, v[0], r[0]);
+        for (int st = 0; st < steps; st += 2) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (st + half < steps) {
+                    if (st + half + 1 < steps) fetch((st + half + 1) * 4, v[1 - half], r[1 - half]);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        if (base + (st + half) * 4 + u < total) {
+                            while (row < r[half][u]) finish();
+                            add_row<T>(acc, v[half][u]);
+                        }
+                    }
+                }
             }
         }
-        TO *o = out + (v0 + r) * ldo + col;
-        float old[EMB_VEC] = {};
-        if (accumulate) load_n<EMB_VEC>(o, D - col, old);
-#pragma unroll
-        for (int i = 0; i < EMB_VEC; ++i) acc[i] = old[i] + scale * acc[i];
-        store_n<EMB_VEC>(o, D - col, acc);
     }
+    while (row < rows) finish();
 }
 
 static inline size_t eal(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -426,23 +541,34 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
     const int lg = emb_lg_tpr(D), rpb = EMB_NT >> lg;
     const int slabs = (D + (EMB_VEC << lg) - 1) / (EMB_VEC << lg);
     if (slabs > 65535) return DDG_E_UNSUPPORTED;
-    const int rows = rpb > 8 ? (rpb < ROWS_MAX ? rpb : ROWS_MAX) : 8;
+    // k_embg_rows: groups of 8 to 64 lanes, and as many rows per group (16 at most, 32 per wave) as leave about 8 192 waves
+    const int rlg = lg < 3 ? 3 : lg > 6 ? 6 : lg, groups = 64 >> rlg;
+    const int64_t rslabs = ceil_div64(D, EMB_VEC << rlg);
+    int64_t rows = V * rslabs / ((int64_t)groups * 8192);
+    const int most = ROWS_MAX / groups < 16 ? ROWS_MAX / groups : 16;
+    rows = rows < 1 ? 1 : rows > most ? most : rows;
+    const int64_t rgrid = ceil_div64(V, EMB_NT / 64 * groups * rows);
+    if (rslabs > 65535) return DDG_E_UNSUPPORTED;
     return ddg_with_type(dy_type, [&](auto ti) {
         using TI = decltype(ti);
-        const int64_t c1 = n / CHUNK1, c2 = n / CHUNK2;
-        if (c1)
-            k_embg_part<TI, 1><<<dim3((unsigned)ceil_div64(c1, rpb), slabs), EMB_NT, 0, s>>>(
-                w.key[cur], w.pos[cur], c1, (uint32_t)V, (const TI *)dy, ld_dy, D, w.part1, lg);
-        if (c2)
-            k_embg_part<float, 2><<<dim3((unsigned)ceil_div64(c2, rpb), slabs), EMB_NT, 0, s>>>(
-                w.key[cur], w.pos[cur], c2, (uint32_t)V, w.part1, D, D, w.part2, lg);
-        return ddg_with_type(out_type, [&](auto to) {
-            using TO = decltype(to);
-            k_embg_rows<TI, TO><<<dim3((unsigned)ceil_div64(V, rows), slabs), EMB_NT, 0, s>>>(
-                w.key[cur], w.pos[cur], n, V, (const TI *)dy, ld_dy, D, w.part1, w.part2, scale, accumulate, (TO *)out, ld_out, lg,
-                rows);
-            DDG_CHECK_LAUNCH();
-            return (int)DDG_OK;
-        });
+        auto sums = [&](auto tiny) {
+            constexpr bool TINY = decltype(tiny)::value;
+            const int64_t c1 = n / CHUNK1, c2 = n / CHUNK2;
+            if (c1)
+                k_embg_part<TI, 1, TINY><<<dim3((unsigned)ceil_div64(c1, rpb), slabs), EMB_NT, 0, s>>>(
+                    w.key[cur], w.pos[cur], c1, (uint32_t)V, (const TI *)dy, ld_dy, D, w.part1, lg);
+            if (c2)
+                k_embg_part<float, 2, TINY><<<dim3((unsigned)ceil_div64(c2, rpb), slabs), EMB_NT, 0, s>>>(
+                    w.key[cur], w.pos[cur], c2, (uint32_t)V, w.part1, D, D, w.part2, lg);
+            return ddg_with_type(out_type, [&](auto to) {
+                using TO = decltype(to);
+                k_embg_rows<TI, TO, TINY><<<dim3((unsigned)rgrid, (unsigned)rslabs), EMB_NT, 0, s>>>(
+                    w.key[cur], w.pos[cur], n, V, (const TI *)dy, ld_dy, D, w.part1, w.part2, scale, accumulate, (TO *)out, ld_out,
+                    rlg, (int)rows);
+                DDG_CHECK_LAUNCH();
+                return (int)DDG_OK;
+            });
+        };
+        return D < EMB_VEC ? sums(std::true_type()) : sums(std::false_type());
     });
 }
