@@ -304,18 +304,17 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_sort_small(const ID *__restric
 // ---------------------------------------------------------------------------------------------
 // sums
 // ---------------------------------------------------------------------------------------------
-// acc += rows [a, b) of src, four rows in flight
+// acc += rows [a, b) of src
 template <bool TINY>
 __device__ __forceinline__ void add_rows(const float *__restrict__ src, const Columns &c, uint32_t a, uint32_t b,
                                          float (&acc)[EMB_VEC]) {
-    vec8<float> v[4];
-    for (; a + 4 <= b; a += 4) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = load_row<TINY>(src + (int64_t)(a + u) * c.D, c);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add_row<float>(acc, v[u]);
+#pragma unroll 1
+    for (; a < b; a += 2) {                             // (two in flight: more would cost every wave registers)
+        const vec8<float> x = load_row<TINY>(src + (int64_t)a * c.D, c);
+        const vec8<float> y = load_row<TINY>(src + (int64_t)(a + 1 < b ? a + 1 : a) * c.D, c);
+        add_row<float>(acc, x);
+        if (a + 1 < b) add_row<float>(acc, y);
     }
-    for (; a < b; ++a) add_row<float>(acc, load_row<TINY>(src + (int64_t)a * c.D, c));
 }
 
 // LEVEL 1: part[c] = sum of the dy rows of sorted positions [64 c, 64 c + 64) if they all belong to one row of the table;
@@ -372,12 +371,13 @@ __device__ __forceinline__ RowParts row_parts(uint32_t a, uint32_t b) {
 // most rows have few tokens, and a walk row by row would wait out the memory's latency for each of them (609 us, now
 // ROWS_US, for 262 144 tokens of 2 048 elements in 128 000 rows).
 template <class T, class TO, bool TINY>
-__global__ __launch_bounds__(EMB_NT) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n,
+__global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n,
                                                       int64_t V, const T *__restrict__ dy, int64_t ld, int D,
                                                       const float *__restrict__ part1, const float *__restrict__ part2, float scale,
-                                                      int accumulate, TO *__restrict__ out, int64_t ldo, int lg, int rows) {
+                                                      int accumulate, TO *__restrict__ out, int64_t ldo, int lg, int rows, int slabs) {
+    const uint32_t rblock = blockIdx.x / slabs, slab = blockIdx.x - rblock * slabs;
     const int lane = threadIdx.x & 63, lanes = 1 << lg, in_group = lane & (lanes - 1), group = lane >> lg;
-    const int64_t wave0 = ((int64_t)blockIdx.x * (EMB_NT / 64) + (threadIdx.x >> 6)) * ((64 >> lg) * rows);
+    const int64_t wave0 = ((int64_t)rblock * (EMB_NT / 64) + (threadIdx.x >> 6)) * ((64 >> lg) * rows);
     if (wave0 >= V) return;
     // lane l: the first sorted position whose key is >= row wave0 + l
     int64_t lo = 0, hi = n;
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(EMB_NT) void k_embg_rows(const uint32_t *__restrict
             if (go && !less) hi = mid;
         }
     }
-    const Columns c((blockIdx.y * lanes + in_group) * EMB_VEC, D);
+    const Columns c((slab * lanes + in_group) * EMB_VEC, D);
     const int64_t v0 = wave0 + group * rows;
     // lane r of the group: row r's positions and single tokens, and how many the rows up to it have.  From here on groups go
     // their own ways and exchange data within themselves only
@@ -429,16 +429,11 @@ __global__ __launch_bounds__(EMB_NT) void k_embg_rows(const uint32_t *__restrict
         ++row;
     };
 
-    vec8<T> v[2][4];
-    int r[2][4];
     int item_pos = 0, item_row = rows;                  // this lane's item of the current batch of `lanes` items
-    auto fetch = [&](int j, vec8<T>(&w)[4], int (&rr)[4]) {
+    auto fetch = [&](int j, vec8<T>(&w)[4]) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {                   // (behind the list: token 0, not used)
-            const int q = __shfl(item_pos, j + u, lanes);
-            rr[u] = __shfl(item_row, j + u, lanes);
-            w[u] = load_row<TINY>(dy + (int64_t)q * ld, c);
-        }
+        for (int u = 0; u < 4; ++u)                     // (behind the list: token 0, not used)
+            w[u] = load_row<TINY>(dy + (int64_t)__shfl(item_pos, j + u, lanes) * ld, c);
     };
     for (int base = 0; base < total; base += lanes) {
         // lane l: item base + l of the list, its row by counting the rows that end before it
@@ -451,22 +446,21 @@ __global__ __launch_bounds__(EMB_NT) void k_embg_rows(const uint32_t *__restrict
         const uint32_t at = ordinal < p.a1 - p.a ? p.a + ordinal : p.b1 + (ordinal - (p.a1 - p.a));
         item_row = it < total ? rr : rows;
         item_pos = it < total ? (int)pos[at] : 0;
-        const int steps = total - base < lanes ? (total - base + 3) / 4 : (lanes + 3) / 4;
-        fetch(0, v[0], r[0]);
-        for (int st = 0; st < steps; st += 2) {
+        const int count = total - base < lanes ? total - base : lanes;
+        vec8<T> v[4], w[4];
+        fetch(0, v);
+        for (int j = 0; j < count; j += 4) {
+            if (j + 4 < count) fetch(j + 4, w);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                if (st + half < steps) {
-                    if (st + half + 1 < steps) fetch((st + half + 1) * 4, v[1 - half], r[1 - half]);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        if (base + (st + half) * 4 + u < total) {
-                            while (row < r[half][u]) finish();
-                            add_row<T>(acc, v[half][u]);
-                        }
-                    }
+            for (int u = 0; u < 4; ++u) {
+                if (j + u < count) {
+                    const int to = __shfl(item_row, j + u, lanes);
+                    while (row < to) finish();
+                    add_row<T>(acc, v[u]);
                 }
             }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = w[u];
         }
     }
     while (row < rows) finish();
@@ -548,7 +542,7 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
     const int most = ROWS_MAX / groups < 16 ? ROWS_MAX / groups : 16;
     rows = rows < 1 ? 1 : rows > most ? most : rows;
     const int64_t rgrid = ceil_div64(V, EMB_NT / 64 * groups * rows);
-    if (rslabs > 65535) return DDG_E_UNSUPPORTED;
+    if (rgrid * rslabs > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
     return ddg_with_type(dy_type, [&](auto ti) {
         using TI = decltype(ti);
         auto sums = [&](auto tiny) {
@@ -562,9 +556,9 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
                     w.key[cur], w.pos[cur], c2, (uint32_t)V, w.part1, D, D, w.part2, lg);
             return ddg_with_type(out_type, [&](auto to) {
                 using TO = decltype(to);
-                k_embg_rows<TI, TO, TINY><<<dim3((unsigned)rgrid, (unsigned)rslabs), EMB_NT, 0, s>>>(
+                k_embg_rows<TI, TO, TINY><<<(unsigned)(rgrid * rslabs), EMB_NT, 0, s>>>(
                     w.key[cur], w.pos[cur], n, V, (const TI *)dy, ld_dy, D, w.part1, w.part2, scale, accumulate, (TO *)out, ld_out,
-                    rlg, (int)rows);
+                    rlg, (int)rows, (int)rslabs);
                 DDG_CHECK_LAUNCH();
                 return (int)DDG_OK;
             });
