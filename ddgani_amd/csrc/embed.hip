@@ -200,21 +200,32 @@ __device__ __forceinline__ uint64_t match_digit(uint32_t d, bool live, int digit
 }
 
 // One wave places the pairs of [lo, hi) in their order; next[digit] is the wave's next free place.  A volatile pointer: the
-// wave's LDS accesses are executed in program order, so the count of one group of 64 is seen by the next.
+// wave's LDS accesses are executed in program order, so the count of one group of 64 is seen by the next.  Four groups are
+// loaded at a time.
 template <class GetK, class GetP, class Put>
 __device__ __forceinline__ void place_segment(int64_t lo, int64_t hi, int shift, int digit_bits, volatile uint32_t *next,
                                               const GetK &getk, const GetP &getp, const Put &put) {
     const int lane = threadIdx.x & 63;
-    for (int64_t g = lo; g < hi; g += 64) {
-        const bool live = g + lane < hi;
-        const uint32_t k = live ? getk(g + lane) : 0, p = live ? getp(g + lane) : 0;
-        const uint32_t d = (k >> shift) & ((1u << digit_bits) - 1);
-        const uint64_t m = match_digit(d, live, digit_bits);
-        const uint32_t rank = __popcll(m & (((uint64_t)1 << lane) - 1));
-        if (live) {
-            const uint32_t at = next[d];
-            put(at + rank, k, p);
-            if (rank == 0) next[d] = at + __popcll(m);
+    for (int64_t g0 = lo; g0 < hi; g0 += 256) {
+        uint32_t k[4], p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = g0 + u * 64 + lane;
+            k[u] = i < hi ? getk(i) : 0;
+            p[u] = i < hi ? getp(i) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (g0 + u * 64 >= hi) break;
+            const bool live = g0 + u * 64 + lane < hi;
+            const uint32_t d = (k[u] >> shift) & ((1u << digit_bits) - 1);
+            const uint64_t m = match_digit(d, live, digit_bits);
+            const uint32_t rank = __popcll(m & (((uint64_t)1 << lane) - 1));
+            if (live) {
+                const uint32_t at = next[d];
+                put(at + rank, k[u], p[u]);
+                if (rank == 0) next[d] = at + __popcll(m);
+            }
         }
     }
 }
@@ -230,15 +241,22 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_scatter(SortSrc<ID> src, int64
     __syncthreads();
     const int64_t lo = blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n, seg = tile / SORT_WAVES;
     const int64_t slo = lo + w * seg < hi ? lo + w * seg : hi, shi = slo + seg < hi ? slo + seg : hi;
-    for (int64_t i = slo + (t & 63); i < shi; i += 64) atomicAdd(&next[w][(src.k(i) >> shift) & (bins - 1)], 1u);
+    for (int64_t i0 = slo + (t & 63); i0 < shi; i0 += 256) {
+        uint32_t k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = i0 + u * 64 < shi ? src.k(i0 + u * 64) : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * 64 < shi) atomicAdd(&next[w][(k[u] >> shift) & (bins - 1)], 1u);
+    }
     uint32_t before = 0, total = 0;
     if (t < bins)
-        for (int b = 0; b < tiles; b += 16) {           // (sixteen loads in flight: a loop of single ones took 30 us)
-            uint32_t h[16];
+        for (int b = 0; b < tiles; b += 32) {           // (32 loads in flight: a loop of single ones took 30 us)
+            uint32_t h[32];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) h[u] = b + u < tiles ? hist[(int64_t)(b + u) * SORT_BINS + t] : 0;
+            for (int u = 0; u < 32; ++u) h[u] = b + u < tiles ? hist[(int64_t)(b + u) * SORT_BINS + t] : 0;
 #pragma unroll
-            for (int u = 0; u < 16; ++u) {
+            for (int u = 0; u < 32; ++u) {
                 total += h[u];
                 if (b + u < (int)blockIdx.x) before += h[u];
             }
