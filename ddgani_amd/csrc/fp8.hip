@@ -433,29 +433,50 @@ __global__ __launch_bounds__(64 * F8_SKW) void k_f8_skinny(const TX *__restrict_
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15;
     const int64_t n0 = (int64_t)blockIdx.x * 16, nr = n0 + m < N ? n0 + m : N - 1;
     const int nk = (int)(kp / F8_BLOCK);
+    const TX *const row = X + (m < M ? m : 0) * ldx;
+    const uint8_t *const brow = B + nr * kp + (lane >> 4) * 32;
     f32x4 acc = {};
-    for (int k = wave; k < nk; k += F8_SKW) {
-        const int64_t c = (int64_t)k * F8_BLOCK + (lane >> 4) * 32;
-        i32x8 fb;
-        __builtin_memcpy(&fb, __builtin_assume_aligned(B + nr * kp + c, 32), 32);
-        const uint32_t eb = Bs[(int64_t)(k >> 2) * N + nr] >> ((k & 3) * 8);
-        float v[32], a = 0.f;
-        load_n<32>(X + (m < M ? m : 0) * ldx + c, m >= M || c >= K ? 0 : K - c >= 32 ? 32 : (int)(K - c), v);
+    typedef TX vec32 __attribute__((ext_vector_type(32)));
+    constexpr int U = sizeof(TX) == 2 ? 4 : 2;          // blocks of the reduction whose loads are in flight together
+    for (int k0 = wave; k0 < nk; k0 += F8_SKW * U) {
+        i32x8 fb[U];
+        uint32_t eb[U];
+        vec32 x[U];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) a = fmaxf(a, fabsf(v[i]));
-        a = fmaxf(a, __shfl_xor(a, 16));
-        a = fmaxf(a, __shfl_xor(a, 32));
-        const int e = f8_exponent(a);
-        const float inv = f8_inverse(e);
-        i32x8 fa;
+        for (int u = 0; u < U; ++u) {                   // (behind the end: the last block again, not used)
+            const int k = k0 + u * F8_SKW < nk ? k0 + u * F8_SKW : nk - 1;
+            const int64_t c = (int64_t)k * F8_BLOCK + (lane >> 4) * 32;
+            __builtin_memcpy(&fb[u], __builtin_assume_aligned(brow + (int64_t)k * F8_BLOCK, 32), 32);
+            eb[u] = Bs[(int64_t)(k >> 2) * N + nr] >> ((k & 3) * 8);
+            if ((k + 1) * (int64_t)F8_BLOCK <= K) {
+                __builtin_memcpy(&x[u], row + c, sizeof(vec32));
+            } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            fa[i] = (int)f8_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
-        bf16x8 xa[4], xb[4];
-        f8_expand(fa, e, xa);
-        f8_expand(fb, eb & 0xFF, xb);
+                for (int i = 0; i < 32; ++i) x[u][i] = c + i < K ? row[c + i] : (TX)0.f;
+            }
+        }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * F8_SKW >= nk) break;
+            float a = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) a = fmaxf(a, fabsf((float)x[u][i]));
+            a = m < M ? a : 0.f;
+            a = fmaxf(a, __shfl_xor(a, 16));
+            a = fmaxf(a, __shfl_xor(a, 32));
+            const int e = f8_exponent(a);
+            const float inv = f8_inverse(e);
+            i32x8 fa;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                fa[i] = (int)f8_pack4((float)x[u][4 * i] * inv, (float)x[u][4 * i + 1] * inv, (float)x[u][4 * i + 2] * inv,
+                                      (float)x[u][4 * i + 3] * inv);
+            bf16x8 xa[4], xb[4];
+            f8_expand(fa, e, xa);
+            f8_expand(fb[u], eb[u] & 0xFF, xb);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
+        }
     }
     part[wave][lane] = acc;
     __syncthreads();
