@@ -89,15 +89,22 @@ __global__ __launch_bounds__(256) void k_f8_pack_rows(const T *__restrict__ x, i
 // F8_ROWS_COLS: those and groups along the rows (q, s); F8_TILE: one scale for the tile, packed both ways (qt may be NULL).
 // sums (may be NULL): fp32 column sums of the tile, [row tile][cols].
 enum { F8_COLS, F8_ROWS_COLS, F8_TILE };
-template <class T, int MODE>
-__global__ __launch_bounds__(256) void k_f8_pack_tile(const T *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, uint8_t *q,
-                                                      uint8_t *s, uint8_t *qt, uint8_t *st, float *sums) {
+struct F8Pack {
+    const void *x;
+    int64_t ld, rows, cols;
+    uint8_t *q, *s, *qt, *st;
+    float *sums;
+};
+template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F8Pack &p, int64_t tile) {
+    const T *const x = (const T *)p.x;
+    const int64_t ld = p.ld, rows = p.rows, cols = p.cols;
+    uint8_t *const q = p.q, *const s = p.s, *const qt = p.qt, *const st = p.st;
+    float *const sums = p.sums;
     __shared__ float red[16][F8_BLOCK];
     __shared__ uint8_t tr[F8_BLOCK][F8_BLOCK + 8];
     const int tc = threadIdx.x & 15, tr8 = (threadIdx.x >> 4) * 8;
-    const int64_t cb = blockIdx.x, rb = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    const int64_t tiles_c = (cols + F8_BLOCK - 1) / F8_BLOCK, rb = tile / tiles_c, cb = tile - rb * tiles_c;
     const int64_t r0 = rb * F8_BLOCK, c0 = cb * F8_BLOCK, c = c0 + tc * 8;
-    if (r0 >= rows) return;
     const int64_t cp = f8_pad(cols), rp = f8_pad(rows);
     const int nc = cols - c >= 8 ? 8 : cols > c ? (int)(cols - c) : 0;
     float v[8][8];
@@ -192,12 +199,27 @@ __global__ __launch_bounds__(256) void k_f8_pack_tile(const T *__restrict__ x, i
     }
 }
 
+template <class T> __global__ __launch_bounds__(256) void k_f8_pack_weight(F8Pack w) { f8_pack_one<T, F8_TILE>(w, blockIdx.x); }
+
+// the operands of both gradients in one launch: tiles of dy, then tiles of x (either may be none)
+template <class T> __global__ __launch_bounds__(256) void k_f8_pack_grads(F8Pack dy, uint32_t tiles_dy, F8Pack x) {
+    if (blockIdx.x < tiles_dy) f8_pack_one<T, F8_ROWS_COLS>(dy, blockIdx.x);
+    else f8_pack_one<T, F8_COLS>(x, blockIdx.x - tiles_dy);
+}
+
+// column sums from those of the row tiles: 64 columns per workgroup, its four waves share the tiles
 __global__ __launch_bounds__(256) void k_f8_colsum(const float *__restrict__ part, int64_t tiles, int64_t cols, float *__restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+    __shared__ float w[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     float a = 0.f;
-    for (int64_t t = 0; t < tiles; ++t) a += part[t * cols + c];
-    out[c] = a;
+    if (c < cols) {
+#pragma unroll 8
+        for (int64_t t = wave; t < tiles; t += 4) a += part[t * cols + c];
+    }
+    w[wave][lane] = a;
+    __syncthreads();
+    if (wave == 0 && c < cols) out[c] = (w[0][lane] + w[1][lane]) + (w[2][lane] + w[3][lane]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -249,27 +271,42 @@ __device__ __forceinline__ void f8_expand(const i32x8 &f, uint32_t e, bf16x8 (&o
 // the barriers do
 __device__ __forceinline__ void f8_copy16(const void *base, uint32_t off, uint32_t dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)((const char *)base + off),
-                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+                                     (__attribute__((address_space(3))) void *)(uintptr_t)dst, 16, 0, 0);
 }
 __device__ __forceinline__ void f8_copy4(const void *base, uint32_t off, uint32_t dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)((const char *)base + off),
-                                     (__attribute__((address_space(3))) void *)dst, 4, 0, 0);
+                                     (__attribute__((address_space(3))) void *)(uintptr_t)dst, 4, 0, 0);
 }
 
-template <int MT, int NT, int WM, int WN, bool EXPAND, class TO>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__restrict__ A, const uint32_t *__restrict__ As,
-                                                             int64_t M, const uint8_t *__restrict__ B,
-                                                             const uint32_t *__restrict__ Bs, int64_t N, int64_t kp,
-                                                             const float *__restrict__ bias, TO *__restrict__ C, int64_t ldc,
-                                                             uint32_t tiles_m, uint32_t tiles_n) {
+struct F8Gemm {
+    const uint8_t *A;
+    const uint32_t *As;
+    int64_t M;
+    const uint8_t *B;
+    const uint32_t *Bs;
+    int64_t N, kp;
+    const float *bias;
+    void *C;
+    int64_t ldc;
+    uint32_t tiles_m, tiles_n;
+};
+
+// tile `id` of the product
+template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __forceinline__ void f8_gemm_tile(const F8Gemm &g, uint32_t id) {
+    const uint8_t *const A = g.A, *const B = g.B;
+    const uint32_t *const As = g.As, *const Bs = g.Bs;
+    const int64_t M = g.M, N = g.N, kp = g.kp, ldc = g.ldc;
+    const float *const bias = g.bias;
+    TO *const C = (TO *)g.C;
+    const uint32_t tiles_m = g.tiles_m, tiles_n = g.tiles_n;
     using S = F8Shape<MT, NT, WM, WN>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Tiles in bands of 8 along m, and every XCD (workgroups go round the eight XCDs) a consecutive run of them: the 32 or
     // more workgroups that share an L2 work on a few rows and columns of tiles
-    const uint32_t tiles = tiles_m * tiles_n, q = tiles / 8, rest = tiles % 8, xcd = blockIdx.x % 8;
-    const uint32_t t = xcd * q + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    const uint32_t tiles = tiles_m * tiles_n, q = tiles / 8, rest = tiles % 8, xcd = id % 8;
+    const uint32_t t = xcd * q + (xcd < rest ? xcd : rest) + id / 8;
     const uint32_t band = t / (8 * tiles_n), in_band = t - band * 8 * tiles_n;
     const uint32_t height = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
     const int64_t m0 = (int64_t)(band * 8 + in_band % height) * S::BM, n0 = (int64_t)(in_band / height) * S::BN;
@@ -419,6 +456,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(const uint8_t *__re
     }
 }
 
+template <int MT, int NT, int WM, int WN, bool EXPAND, class TO>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Gemm g) {
+    f8_gemm_tile<MT, NT, WM, WN, EXPAND, TO>(g, blockIdx.x);
+}
+// dW (fp32) and dX of one layer in one launch: neither has the tiles for whole rounds of the CUs.  dW's, the longer ones, first
+template <bool EXPAND, class TO> __global__ __launch_bounds__(256, 2) void k_f8_gemm_grads(F8Gemm dw, F8Gemm dx) {
+    const uint32_t first = dw.tiles_m * dw.tiles_n;
+    if (blockIdx.x < first) f8_gemm_tile<4, 4, 2, 2, true, float>(dw, blockIdx.x);
+    else f8_gemm_tile<4, 4, 2, 2, EXPAND, TO>(dx, blockIdx.x - first);
+}
+
 // At most 16 rows: bound by the bytes of B.  A workgroup owns 16 rows of B and its eight waves share the reduction; the
 // rows of X are quantised on the way (each lane its 32 elements of a group), so one launch does the layer.  Every result
 // type takes the expanded product here: the matrix unit is idle either way.
@@ -514,46 +562,63 @@ static int f8_pack_rows(const void *x, int type, int64_t ld, const F8Operand &o,
         return (int)DDG_OK;
     });
 }
-// x [rows, cols] -> o (groups along rows, or tiles) and ot (its transpose); see k_f8_pack_tile
-template <int MODE>
-static int f8_pack_tile(const void *x, int type, int64_t ld, int64_t rows, int64_t cols, const F8Operand &o, const F8Operand &ot,
-                        float *sums, hipStream_t s) {
-    const int64_t rb = ceil_div64(rows, F8_BLOCK), cb = ceil_div64(cols, F8_BLOCK), gy = rb < 32768 ? rb : 32768;
-    const dim3 grid((unsigned)cb, (unsigned)gy, (unsigned)ceil_div64(rb, gy));
-    return ddg_with_type(type, [&](auto t) {
-        using T = decltype(t);
-        k_f8_pack_tile<T, MODE><<<grid, 256, 0, s>>>((const T *)x, ld, rows, cols, o.q, o.s, ot.q, ot.s, sums);
-        DDG_CHECK_LAUNCH();
-        return (int)DDG_OK;
-    });
-}
+static inline int64_t f8_tiles(int64_t rows, int64_t cols) { return ceil_div64(rows, F8_BLOCK) * ceil_div64(cols, F8_BLOCK); }
 
 // reductions are addressed with 32-bit offsets within a workgroup's 256 rows
 #define F8_MAX_REDUCTION ((int64_t)1 << 24)
 
+template <class S>
+static int f8_problem(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int64_t ldc, F8Gemm &g) {
+    const int64_t tm = ceil_div64(a.rows, S::BM), tn = ceil_div64(b.rows, S::BN), kp = f8_pad(a.cols);
+    if (kp >= F8_MAX_REDUCTION || tm * tn > 0x0FFFFFFF) return DDG_E_UNSUPPORTED;
+    g = {a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s, b.rows, kp, bias, c, ldc, (uint32_t)tm, (uint32_t)tn};
+    return DDG_OK;
+}
+template <class K> static int f8_lds(K kernel, int bytes) {
+    return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? DDG_OK
+                                                                                                                 : DDG_E_LAUNCH;
+}
+// 256 x 256 tiles once there are three quarters of a CU's worth of them, else 128 x 128
+static inline bool f8_wide(int64_t rows_a, int64_t rows_b) { return ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256) >= 192; }
+
 static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int type, int64_t ldc, hipStream_t s) {
-    if (f8_pad(a.cols) >= F8_MAX_REDUCTION) return DDG_E_UNSUPPORTED;
     return ddg_with_type(type, [&](auto t) {
         using TO = decltype(t);
         constexpr bool EXPAND = !std::is_same<TO, bf16_t>::value;
         auto go = [&](auto mt, auto nt, auto wm, auto wn) {
             constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
             using S = F8Shape<MT, NT, WM, WN>;
-            const int64_t tm = ceil_div64(a.rows, S::BM), tn = ceil_div64(b.rows, S::BN);
-            if (tm * tn > 0x0FFFFFFF) return (int)DDG_E_UNSUPPORTED;
+            F8Gemm g;
+            int rc = f8_problem<S>(a, b, bias, c, ldc, g);
             const auto kernel = k_f8_gemm<MT, NT, WM, WN, EXPAND, TO>;
-            if (hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    S::LDS(sizeof(TO))) != hipSuccess)
-                return (int)DDG_E_LAUNCH;
-            kernel<<<(unsigned)(tm * tn), 64 * WM * WN, S::LDS(sizeof(TO)), s>>>(a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s,
-                                                                     b.rows, f8_pad(a.cols), bias, (TO *)c, ldc, (uint32_t)tm,
-                                                                     (uint32_t)tn);
+            if (rc || (rc = f8_lds(kernel, S::LDS(sizeof(TO))))) return rc;
+            kernel<<<g.tiles_m * g.tiles_n, 64 * WM * WN, S::LDS(sizeof(TO)), s>>>(g);
             DDG_CHECK_LAUNCH();
             return (int)DDG_OK;
         };
         if constexpr (!EXPAND)
-            if (ceil_div64(a.rows, 256) * ceil_div64(b.rows, 256) >= 192) return go(Int<8>(), Int<4>(), Int<2>(), Int<4>());
+            if (f8_wide(a.rows, b.rows)) return go(Int<8>(), Int<4>(), Int<2>(), Int<4>());
         return go(Int<4>(), Int<4>(), Int<2>(), Int<2>());
+    });
+}
+
+// dx = gy wt, dw = gyt xt
+static int f8_gemm_grads(const F8Operand &gy, const F8Operand &wt, void *dx, int dx_type, int64_t ld_dx, const F8Operand &gyt,
+                         const F8Operand &xt, float *dw, hipStream_t s) {
+    if (dx_type == DDG_BF16 && f8_wide(gy.rows, wt.rows)) {
+        const int rc = f8_gemm(gy, wt, nullptr, dx, dx_type, ld_dx, s);
+        return rc ? rc : f8_gemm(gyt, xt, nullptr, dw, DDG_F32, xt.rows, s);
+    }
+    return ddg_with_type(dx_type, [&](auto t) {
+        using TO = decltype(t);
+        using S = F8Shape<4, 4, 2, 2>;
+        F8Gemm gw, gx;
+        const auto kernel = k_f8_gemm_grads<!std::is_same<TO, bf16_t>::value, TO>;
+        int rc = f8_problem<S>(gyt, xt, nullptr, dw, xt.rows, gw);
+        if (rc || (rc = f8_problem<S>(gy, wt, nullptr, dx, ld_dx, gx)) || (rc = f8_lds(kernel, S::LDS(4)))) return rc;
+        kernel<<<gw.tiles_m * gw.tiles_n + gx.tiles_m * gx.tiles_n, 256, S::LDS(4), s>>>(gw, gx);
+        DDG_CHECK_LAUNCH();
+        return (int)DDG_OK;
     });
 }
 
@@ -563,7 +628,15 @@ extern "C" int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t 
     if (((uintptr_t)packed | (uintptr_t)packed_t) & 255) return DDG_E_ARG;
     F8Operand t = {};
     if (packed_t) t = f8_operand(packed_t, in, out);
-    return f8_pack_tile<F8_TILE>(W, type, ld, out, in, f8_operand(packed, out, in), t, nullptr, (hipStream_t)stream);
+    const F8Operand o = f8_operand(packed, out, in);
+    const int64_t tiles = f8_tiles(out, in);
+    if (tiles > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
+    return ddg_with_type(type, [&](auto ty) {
+        k_f8_pack_weight<decltype(ty)><<<(unsigned)tiles, 256, 0, (hipStream_t)stream>>>(
+            F8Pack{W, ld, out, in, o.q, o.s, t.q, t.s, nullptr});
+        DDG_CHECK_LAUNCH();
+        return (int)DDG_OK;
+    });
 }
 
 extern "C" size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t in) {
@@ -637,14 +710,24 @@ extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, 
     const F8GradWs w = f8_grad_carve(workspace, rows, out, in);
     const hipStream_t s = (hipStream_t)stream;
     const F8Operand gy = f8_operand(w.dy, rows, out), gyt = f8_operand(w.dyt, out, rows), xt = f8_operand(w.xt, in, rows);
-    int rc = f8_pack_tile<F8_ROWS_COLS>(dy, dy_type, ld_dy, rows, out, gy, gyt, db ? w.sums : nullptr, s);
+    const int64_t tiles_dy = f8_tiles(rows, out), tiles_x = f8_tiles(rows, in), row_tiles = ceil_div64(rows, F8_BLOCK);
+    if (tiles_dy + tiles_x > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
+    // (one row tile: its column sums are the result)
+    const F8Pack pd = {dy, ld_dy, rows, out, gy.q, gy.s, gyt.q, gyt.s, !db ? nullptr : row_tiles == 1 ? db : w.sums};
+    const F8Pack px = {x, ld_x, rows, in, nullptr, nullptr, xt.q, xt.s, nullptr};
+    auto pack = [&](int type, int64_t td, int64_t tx) {
+        return ddg_with_type(type, [&](auto t) {
+            k_f8_pack_grads<decltype(t)><<<(unsigned)(td + tx), 256, 0, s>>>(pd, (uint32_t)td, px);
+            DDG_CHECK_LAUNCH();
+            return (int)DDG_OK;
+        });
+    };
+    int rc = pack(dy_type, tiles_dy, x_type == dy_type ? tiles_x : 0);
+    if (!rc && x_type != dy_type) rc = pack(x_type, 0, tiles_x);
     if (rc) return rc;
-    if (db) {
-        k_f8_colsum<<<(unsigned)ceil_div64(out, 256), 256, 0, s>>>(w.sums, ceil_div64(rows, F8_BLOCK), out, db);
+    if (db && row_tiles > 1) {
+        k_f8_colsum<<<(unsigned)ceil_div64(out, 64), 256, 0, s>>>(w.sums, row_tiles, out, db);
         DDG_CHECK_LAUNCH();
     }
-    rc = f8_pack_tile<F8_COLS>(x, x_type, ld_x, rows, in, F8Operand{}, xt, nullptr, s);
-    if (rc) return rc;
-    rc = f8_gemm(gy, f8_operand((void *)packed_wt, in, out), nullptr, dx, dx_type, ld_dx, s);
-    return rc ? rc : f8_gemm(gyt, xt, nullptr, dw, DDG_F32, in, s);
+    return f8_gemm_grads(gy, f8_operand((void *)packed_wt, in, out), dx, dx_type, ld_dx, gyt, xt, dw, s);
 }
