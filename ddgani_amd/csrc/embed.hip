@@ -23,14 +23,13 @@ struct Columns {
     int col, at, D;
     __device__ Columns(int c, int d) : col(c), at(c < d - EMB_VEC ? c : d > EMB_VEC ? d - EMB_VEC : 0), D(d) {}
 };
-template <class T> using vec8 = T __attribute__((ext_vector_type(EMB_VEC)));
 template <bool TINY, class T> __device__ __forceinline__ vec8<T> load_row(const T *row, const Columns &c) {
     vec8<T> v;
     if (TINY) {
 #pragma unroll
         for (int i = 0; i < EMB_VEC; ++i) v[i] = i < c.D ? row[i] : (T)0.f;
     } else {
-        __builtin_memcpy(&v, row + c.at, sizeof(v));
+        v = load_whole(row + c.at);
     }
     return v;
 }

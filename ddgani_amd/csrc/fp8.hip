@@ -358,7 +358,7 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     i32x8 fa[MT], fb;
     uint32_t ea[MT], eb;
     constexpr int HALF = S::LOADS / 2, EVERY = HALF < MT ? MT / HALF : 1;
-    static_assert(S::LOADS % 2 == 0 && HALF * EVERY == MT, "half a stage's copies in a column of tiles");
+    static_assert(S::LOADS % 2 == 0 && HALF * EVERY <= MT, "half a stage's copies in a column of tiles");
 #pragma unroll
     for (int i = 0; i <= S::LOADS; ++i) copy(0, 0, i);
 #pragma unroll
@@ -404,11 +404,11 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
                 if (j + 1 == NT) {
                     fa[i] = frag(lo_a, hi_a, k + 1, i);
                     ea[i] = scale(sc_a, k + 1, i);
-                    if (i % EVERY == EVERY - 1) copy(k + 2 < nk ? k + 2 : nk - 1, k & 1, i / EVERY);
+                    if (i % EVERY == EVERY - 1 && i / EVERY < HALF) copy(k + 2 < nk ? k + 2 : nk - 1, k & 1, i / EVERY);
                     __builtin_amdgcn_sched_barrier(0);  // not earlier: the register is in use until here
                 }
                 if (j == 0) {
-                    if (i % EVERY == EVERY - 1) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, HALF + i / EVERY);
+                    if (i % EVERY == EVERY - 1 && i / EVERY < HALF) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, HALF + i / EVERY);
                     if (i == MT - 1) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, S::LOADS);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -467,70 +467,99 @@ template <bool EXPAND, class TO> __global__ __launch_bounds__(256, 2) void k_f8_
     else f8_gemm_tile<4, 4, 2, 2, EXPAND, TO>(dx, blockIdx.x - first);
 }
 
-// At most 16 rows: bound by the bytes of B.  A workgroup owns 16 rows of B and its eight waves share the reduction; the
-// rows of X are quantised on the way (each lane its 32 elements of a group), so one launch does the layer.  Every result
-// type takes the expanded product here: the matrix unit is idle either way.
+// At most 16 rows: bound by the bytes of B and by latency, so one launch does the layer.  A workgroup owns 16 rows of B; its W
+// waves share the reduction, and their first codes of B are on the way while the workgroup quantises X into LDS (in pieces
+// of the reduction that fit), each element once: quantised by the lanes that multiply it, 16 rows at a time whatever their
+// number, X took longer than B.  Every result type takes the expanded product here: the matrix unit is idle either way.
 #define F8_SKINNY 16
-#define F8_SKW 8
-template <class TX, class TO>
-__global__ __launch_bounds__(64 * F8_SKW) void k_f8_skinny(const TX *__restrict__ X, int64_t ldx, int M, int64_t K,
-                                                           const uint8_t *__restrict__ B, const uint32_t *__restrict__ Bs, int64_t N,
-                                                           int64_t kp, const float *__restrict__ bias, TO *__restrict__ C,
-                                                           int64_t ldc) {
-    __shared__ f32x4 part[F8_SKW][64];
+#define F8_SKINNY_LDS (140 * 1024)
+template <class TX, class TO, int W>
+__global__ __launch_bounds__(64 * W) void k_f8_skinny(const TX *__restrict__ X, int64_t ldx, int M, int64_t K, const uint8_t *__restrict__ B,
+                                                      const uint32_t *__restrict__ Bs, int64_t N, int64_t kp,
+                                                      const float *__restrict__ bias, TO *__restrict__ C, int64_t ldc, int piece) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];       // [M][pitch] codes, [M][piece] exponents, [W][64] sums
+    constexpr int U = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15;
     const int64_t n0 = (int64_t)blockIdx.x * 16, nr = n0 + m < N ? n0 + m : N - 1;
-    const int nk = (int)(kp / F8_BLOCK);
-    const TX *const row = X + (m < M ? m : 0) * ldx;
+    const int nk = (int)(kp / F8_BLOCK), pitch = piece * F8_BLOCK + 16;
+    uint8_t *const ex = lds + M * pitch;
     const uint8_t *const brow = B + nr * kp + (lane >> 4) * 32;
     f32x4 acc = {};
-    typedef TX vec32 __attribute__((ext_vector_type(32)));
-    constexpr int U = sizeof(TX) == 2 ? 4 : 2;          // blocks of the reduction whose loads are in flight together
-    for (int k0 = wave; k0 < nk; k0 += F8_SKW * U) {
-        i32x8 fb[U];
-        uint32_t eb[U];
-        vec32 x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {                   // (behind the end: the last block again, not used)
-            const int k = k0 + u * F8_SKW < nk ? k0 + u * F8_SKW : nk - 1;
-            const int64_t c = (int64_t)k * F8_BLOCK + (lane >> 4) * 32;
-            __builtin_memcpy(&fb[u], __builtin_assume_aligned(brow + (int64_t)k * F8_BLOCK, 32), 32);
-            eb[u] = Bs[(int64_t)(k >> 2) * N + nr] >> ((k & 3) * 8);
-            if ((k + 1) * (int64_t)F8_BLOCK <= K) {
-                __builtin_memcpy(&x[u], row + c, sizeof(vec32));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[u][i] = c + i < K ? row[c + i] : (TX)0.f;
-            }
-        }
+    i32x8 fb[U];
+    uint32_t eb[U];
+    auto load = [&](int k0) {                           // blocks k0, k0 + W, ... (behind the end: the last block, not used)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (k0 + u * F8_SKW >= nk) break;
-            float a = 0.f;
+            const int k = k0 + u * W < nk ? k0 + u * W : nk - 1;
+            __builtin_memcpy(&fb[u], __builtin_assume_aligned(brow + (int64_t)k * F8_BLOCK, 32), 32);
+            eb[u] = Bs[(int64_t)(k >> 2) * N + nr] >> ((k & 3) * 8);
+        }
+    };
+    for (int p0 = 0; p0 < nk; p0 += piece) {
+        const int here = nk - p0 < piece ? nk - p0 : piece;
+        load(p0 + wave);
+        if (p0) __syncthreads();                        // the last piece has been read
+        auto quantise = [&](auto in_flight) {           // groups of 128 of this lane's 16, that many loaded at a time
+            constexpr int Q = decltype(in_flight)::value;
+            for (int g0 = threadIdx.x >> 4; g0 < M * here; g0 += W * 4 * Q) {
+                vec8<TX> v[Q];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) a = fmaxf(a, fabsf((float)x[u][i]));
-            a = m < M ? a : 0.f;
-            a = fmaxf(a, __shfl_xor(a, 16));
-            a = fmaxf(a, __shfl_xor(a, 32));
-            const int e = f8_exponent(a);
-            const float inv = f8_inverse(e);
-            i32x8 fa;
+                for (int u = 0; u < Q; ++u) {
+                    const int g = g0 + u * W * 4, row = g / here, k = g - row * here;
+                    const int64_t c = (int64_t)(p0 + k) * F8_BLOCK + m * 8;
+                    const TX *p = X + (row < M ? row : 0) * ldx;
+                    if (K >= 8) v[u] = load_whole(p + (c + 8 <= K ? c : 0));
+                    if (K % 8 && c < K && c + 8 > K) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                fa[i] = (int)f8_pack4((float)x[u][4 * i] * inv, (float)x[u][4 * i + 1] * inv, (float)x[u][4 * i + 2] * inv,
-                                      (float)x[u][4 * i + 3] * inv);
-            bf16x8 xa[4], xb[4];
-            f8_expand(fa, e, xa);
-            f8_expand(fb[u], eb[u] & 0xFF, xb);
+                        for (int i = 0; i < 8; ++i) v[u][i] = c + i < K ? p[c + i] : (TX)0.f;
+                    }
+                }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
+                for (int u = 0; u < Q; ++u) {
+                    const int g = g0 + u * W * 4, row = g / here, k = g - row * here;
+                    if (g >= M * here) break;           // (whole groups of 16 lanes leave)
+                    const bool live = (int64_t)(p0 + k) * F8_BLOCK + m * 8 < K;
+                    float f[8], a = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        f[i] = live ? (float)v[u][i] : 0.f;
+                        a = fmaxf(a, fabsf(f[i]));
+                    }
+                    const int e = f8_exponent(row16_max(a));
+                    const float inv = f8_inverse(e);
+                    uint2 w;
+                    w.x = f8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+                    w.y = f8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+                    *(uint2 *)(lds + row * pitch + k * F8_BLOCK + m * 8) = w;
+                    if (m == 0) ex[row * piece + k] = (uint8_t)e;
+                }
+            }
+        };
+        if (M * here <= W * 4) quantise(std::integral_constant<int, 1>());
+        else quantise(std::integral_constant<int, 4>());
+        __syncthreads();
+        const uint8_t *const arow = lds + (m < M ? m : 0) * pitch + (lane >> 4) * 32, *const erow = ex + (m < M ? m : 0) * piece;
+        for (int k0 = wave; k0 < here; k0 += U * W) {
+            if (k0 != wave) load(p0 + k0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = k0 + u * W;
+                if (k >= here) break;
+                const i32x4 x = *(const i32x4 *)(arow + k * F8_BLOCK), y = *(const i32x4 *)(arow + k * F8_BLOCK + 16);
+                bf16x8 xa[4], xb[4];
+                f8_expand(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), erow[k], xa);
+                f8_expand(fb[u], eb[u] & 0xFF, xb);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
+            }
         }
     }
-    part[wave][lane] = acc;
+    f32x4 *const part = (f32x4 *)(lds + ((M * (pitch + piece) + 15) & ~15));
+    part[wave * 64 + lane] = acc;
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int w = 1; w < F8_SKW; ++w) acc += part[w][lane];
+    for (int w = 1; w < W; ++w) acc += part[w * 64 + lane];
     const int64_t n = n0 + (lane >> 4) * 4;
     const int left = N - n >= 4 ? 4 : N > n ? (int)(N - n) : 0;
     if (m >= M) return;
@@ -659,10 +688,21 @@ extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t r
             return ddg_with_type(y_type, [&](auto to) {
                 using TX = decltype(tx);
                 using TO = decltype(to);
-                k_f8_skinny<TX, TO><<<(unsigned)ceil_div64(out, 16), 64 * F8_SKW, 0, s>>>(
-                    (const TX *)x, ld_x, (int)rows, in, w.q, (const uint32_t *)w.s, out, f8_pad(in), bias, (TO *)y, ld_y);
-                DDG_CHECK_LAUNCH();
-                return (int)DDG_OK;
+                const int nk = (int)(f8_pad(in) / F8_BLOCK), most = F8_SKINNY_LDS / (F8_BLOCK + 1) / (int)rows;
+                auto go = [&](auto waves) {
+                    constexpr int W = decltype(waves)::value;
+                    const int piece = nk < most ? nk : most / W * W;        // (a wave's blocks stay its own from piece to piece)
+                    const int bytes = (((int)rows * (piece * (F8_BLOCK + 1) + 16) + 15) & ~15) + W * 64 * 16;
+                    const auto kernel = k_f8_skinny<TX, TO, W>;
+                    const int rc = f8_lds(kernel, bytes);
+                    if (rc) return rc;
+                    kernel<<<(unsigned)ceil_div64(out, 16), 64 * W, bytes, s>>>((const TX *)x, ld_x, (int)rows, in, w.q,
+                                                                               (const uint32_t *)w.s, out, f8_pad(in), bias, (TO *)y,
+                                                                               ld_y, piece);
+                    DDG_CHECK_LAUNCH();
+                    return (int)DDG_OK;
+                };
+                return nk > 8 ? go(Int<16>()) : go(Int<8>());
             });
         });
     if (!workspace || workspace_bytes < ddg_fp8_linear_workspace_bytes(rows, in)) return DDG_E_WORKSPACE;

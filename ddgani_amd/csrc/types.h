@@ -45,6 +45,14 @@ template <int N, class T> __device__ __forceinline__ void store_n(T *p, int n, c
     }
 }
 
+// eight consecutive elements, all of them in bounds: one load without a branch around it
+template <class T> using vec8 = T __attribute__((ext_vector_type(8)));
+template <class T> __device__ __forceinline__ vec8<T> load_whole(const T *p) {
+    vec8<T> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+
 // maximum over the 16 lanes of a DPP row, in every lane
 __device__ __forceinline__ float row16_max(float x) {
 #define DDG_DPP_MAX(ctrl)                                                                                                   \
