@@ -170,7 +170,7 @@ SIGNATURES = {
                                  C.c_size_t, C.c_void_p]),
     "ddg_fp8_operand_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
     "ddg_fp8_pack_weight": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "ddg_fp8_linear_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "ddg_fp8_linear_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
     "ddg_fp8_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, c_f32p, C.c_void_p,
                                  C.c_int, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
     "ddg_fp8_linear_grads_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),

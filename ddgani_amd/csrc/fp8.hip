@@ -246,7 +246,7 @@ template <int MT, int NT, int WM, int WN> struct F8Shape {
     static constexpr int PITCH(int bytes) { return NT * 16 * bytes + 16; }
     static constexpr int OUT(int bytes) { return MT * 16 * PITCH(bytes); }
     static constexpr int LDS(int bytes) { return STAGES > WAVES * OUT(bytes) ? STAGES : WAVES * OUT(bytes); }
-    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && ROWS == 64 * WAVES && BM % 64 == 0,
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && ROWS % 64 == 0 && ROWS <= 64 * WAVES && BM % 64 == 0,
                   "whole copies: eight rows of codes, 64 rows of scale words per wave");
 };
 
@@ -289,16 +289,19 @@ struct F8Gemm {
     void *C;
     int64_t ldc;
     uint32_t tiles_m, tiles_n;
+    uint32_t splits, blocks;            // the reduction in `splits` parts of `blocks` (a multiple of 4) blocks; part s goes to
+                                        // C + s * M * N (fp32, dense), k_f8_join adds the parts
 };
 
 // tile `id` of the product
 template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __forceinline__ void f8_gemm_tile(const F8Gemm &g, uint32_t id) {
-    const uint8_t *const A = g.A, *const B = g.B;
-    const uint32_t *const As = g.As, *const Bs = g.Bs;
-    const int64_t M = g.M, N = g.N, kp = g.kp, ldc = g.ldc;
+    const uint32_t tiles_m = g.tiles_m, tiles_n = g.tiles_n, split = id / (tiles_m * tiles_n);
+    id -= split * tiles_m * tiles_n;
+    const int64_t M = g.M, N = g.N, kp = g.kp, ldc = g.ldc, k0 = (int64_t)split * g.blocks;
+    const uint8_t *const A = g.A + k0 * F8_BLOCK, *const B = g.B + k0 * F8_BLOCK;
+    const uint32_t *const As = g.As + k0 / 4 * M, *const Bs = g.Bs + k0 / 4 * N;
     const float *const bias = g.bias;
-    TO *const C = (TO *)g.C;
-    const uint32_t tiles_m = g.tiles_m, tiles_n = g.tiles_n;
+    TO *const C = (TO *)g.C + split * M * N;
     using S = F8Shape<MT, NT, WM, WN>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
@@ -311,7 +314,7 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     const uint32_t height = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
     const int64_t m0 = (int64_t)(band * 8 + in_band % height) * S::BM, n0 = (int64_t)(in_band / height) * S::BN;
     const int wm = (wave % WM) * (MT * 16), wn = (wave / WM) * (NT * 16);
-    const int nk = (int)(kp / F8_BLOCK);
+    const int nk = (int)(kp / F8_BLOCK - k0 < g.blocks ? kp / F8_BLOCK - k0 : g.blocks);
 
     const uint8_t *const a0 = A + m0 * kp, *const b0 = B + n0 * kp;
     const int64_t rows_a = M - m0, rows_b = N - n0;
@@ -322,8 +325,9 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
         const int64_t last = (i < S::LOADS_A ? rows_a : rows_b) - 1;
         off[i] = (uint32_t)(row < last ? row : last) * (uint32_t)kp + (((lane & 7) ^ f8_swap(in)) * 16);
     }
-    const bool scale_a = wave * 64 < S::BM;
-    const uint32_t *const s0 = scale_a ? As + m0 + wave * 64 : Bs + n0 + (wave * 64 - S::BM);
+    const int srow = (wave < S::ROWS / 64 ? wave : S::ROWS / 64 - 1) * 64;        // (further waves copy the last piece again)
+    const bool scale_a = srow < S::BM;
+    const uint32_t *const s0 = scale_a ? As + m0 + srow : Bs + n0 + (srow - S::BM);
     const int64_t s_rows = scale_a ? M : N;
     // piece i of stage k to buffer buf; the scale words are piece LOADS, copied with each of their four stages (the same bytes
     // over themselves).  No branches around here: the compiler would move matrix instructions across them
@@ -336,7 +340,7 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
         } else {                                        // (an operand's scales are followed by 1 KB that may be read)
             const uint32_t *base = s0 + (k >> 2) * s_rows;
             asm("" : "+s"(base));
-            f8_copy4(base, lane * 4, lds0 + 2 * S::STAGE + ((k >> 2) & 1) * (S::ROWS * 4) + wave * 256);
+            f8_copy4(base, lane * 4, lds0 + 2 * S::STAGE + ((k >> 2) & 1) * (S::ROWS * 4) + srow * 4);
         }
     };
     // this lane's two pieces of a fragment (row lane % 16 of a tile, 32 codes of the block) and its scale, for the wave's
@@ -457,14 +461,43 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
 }
 
 template <int MT, int NT, int WM, int WN, bool EXPAND, class TO>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Gemm g) {
+__global__ __launch_bounds__(64 * WM * WN, MT * NT <= 8 ? 3 : 2) void k_f8_gemm(F8Gemm g) {
     f8_gemm_tile<MT, NT, WM, WN, EXPAND, TO>(g, blockIdx.x);
 }
 // dW (fp32) and dX of one layer in one launch: neither has the tiles for whole rounds of the CUs.  dW's, the longer ones, first
-template <bool EXPAND, class TO> __global__ __launch_bounds__(256, 2) void k_f8_gemm_grads(F8Gemm dw, F8Gemm dx) {
-    const uint32_t first = dw.tiles_m * dw.tiles_n;
-    if (blockIdx.x < first) f8_gemm_tile<4, 4, 2, 2, true, float>(dw, blockIdx.x);
-    else f8_gemm_tile<4, 4, 2, 2, EXPAND, TO>(dx, blockIdx.x - first);
+template <int NT, bool EXPAND, class TO> __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void k_f8_gemm_grads(F8Gemm dw, F8Gemm dx) {
+    const uint32_t first = dw.tiles_m * dw.tiles_n * dw.splits;
+    if (blockIdx.x < first) f8_gemm_tile<4, NT, 2, 2, true, float>(dw, blockIdx.x);
+    else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, blockIdx.x - first);
+}
+
+// C = bias + sum of the parts, in their order; four columns per thread
+struct F8Join {
+    const float *part;
+    int64_t M, N;
+    uint32_t splits;
+    const float *bias;
+    void *C;
+    int64_t ldc;
+};
+template <class TO> __device__ __forceinline__ void f8_join(const F8Join &j, int64_t i) {
+    const int64_t units = (j.N + 3) / 4, m = i / units, n = (i - m * units) * 4;
+    if (m >= j.M) return;
+    const int left = j.N - n < 4 ? (int)(j.N - n) : 4;
+    float v[4] = {}, p[4];
+    if (j.bias) load_n<4>(j.bias + n, left, v);
+#pragma unroll 4
+    for (uint32_t s = 0; s < j.splits; ++s) {
+        load_n<4>(j.part + (s * j.M + m) * j.N + n, left, p);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] += p[u];
+    }
+    store_n<4>((TO *)j.C + m * j.ldc + n, left, v);
+}
+// a: of type TO, `first` workgroups; b: fp32 (either may be none)
+template <class TO> __global__ __launch_bounds__(256) void k_f8_join(F8Join a, uint32_t first, F8Join b) {
+    if (blockIdx.x < first) f8_join<TO>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
+    else f8_join<float>(b, (int64_t)(blockIdx.x - first) * 256 + threadIdx.x);
 }
 
 // At most 16 rows: bound by the bytes of B and by latency, so one launch does the layer.  A workgroup owns 16 rows of B; its W
@@ -596,59 +629,135 @@ static inline int64_t f8_tiles(int64_t rows, int64_t cols) { return ceil_div64(r
 // reductions are addressed with 32-bit offsets within a workgroup's 256 rows
 #define F8_MAX_REDUCTION ((int64_t)1 << 24)
 
+// Tiles are 256 x 256 (bf16 results only) once there are three quarters of a CU's worth of them; else 128 x 128, or 128 x 64 while
+// all tiles together have fewer than eight stages for each of 512 workgroups: there the time is latency.  A tile whose reduction
+// takes twice its share of all stages and more is split into parts of about that share (a whole number of scale words, so
+// four stages at least), which are added afterwards, where that saves more (0.6 us a stage) than it costs (a launch, 3 us, and
+// the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 13.7 us, 128 x 4096 x 4096
+// 36 -> 24 us; 256 x 1000 x 8192 would go from 16 to 21 us and is left whole.
+#define F8_WORKGROUPS 512
+static inline bool f8_wide(int64_t rows_a, int64_t rows_b) { return ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256) >= 192; }
+static inline int64_t f8_stages(int64_t rows_a, int64_t rows_b, int64_t cols, int bn) {
+    return ceil_div64(rows_a, 128) * ceil_div64(rows_b, bn) * (f8_pad(cols) / F8_BLOCK);
+}
+struct F8Split {
+    int64_t splits, blocks;
+};
+static inline F8Split f8_split(int64_t m, int64_t n, int64_t cols, int64_t all_stages) {
+    const int64_t nk = f8_pad(cols) / F8_BLOCK, share = ceil_div64(ceil_div64(all_stages, F8_WORKGROUPS), 4) * 4;
+    const int64_t splits = ceil_div64(nk, share);
+    if (nk < 2 * share || (nk - share) * 600 < 3000 + splits * m * n / 800) return {1, ceil_div64(nk, 4) * 4};
+    return {splits, share};
+}
+// the split of a product on its own
+static inline F8Split f8_split_one(int64_t rows_a, int64_t rows_b, int64_t cols, bool bf16) {
+    if (bf16 && f8_wide(rows_a, rows_b)) return {1, ceil_div64(f8_pad(cols) / F8_BLOCK, 4) * 4};
+    const bool narrow = f8_stages(rows_a, rows_b, cols, 128) < 8 * F8_WORKGROUPS;
+    return f8_split(rows_a, rows_b, cols, f8_stages(rows_a, rows_b, cols, narrow ? 64 : 128));
+}
+static inline size_t f8_parts_bytes(const F8Split &sp, int64_t m, int64_t n) {
+    return sp.splits > 1 ? ((size_t)sp.splits * m * n * 4 + 255) & ~(size_t)255 : 0;
+}
+
 template <class S>
-static int f8_problem(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int64_t ldc, F8Gemm &g) {
+static int f8_problem(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int64_t ldc, const F8Split &sp, float *parts,
+                      F8Gemm &g) {
     const int64_t tm = ceil_div64(a.rows, S::BM), tn = ceil_div64(b.rows, S::BN), kp = f8_pad(a.cols);
-    if (kp >= F8_MAX_REDUCTION || tm * tn > 0x0FFFFFFF) return DDG_E_UNSUPPORTED;
-    g = {a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s, b.rows, kp, bias, c, ldc, (uint32_t)tm, (uint32_t)tn};
+    if (kp >= F8_MAX_REDUCTION || tm * tn * sp.splits > 0x0FFFFFFF) return DDG_E_UNSUPPORTED;
+    const bool split = sp.splits > 1;
+    g = {a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s, b.rows, kp, split ? nullptr : bias, split ? parts : c,
+         split ? b.rows : ldc, (uint32_t)tm, (uint32_t)tn, (uint32_t)sp.splits, (uint32_t)sp.blocks};
     return DDG_OK;
 }
 template <class K> static int f8_lds(K kernel, int bytes) {
     return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? DDG_OK
                                                                                                                  : DDG_E_LAUNCH;
 }
-// 256 x 256 tiles once there are three quarters of a CU's worth of them, else 128 x 128
-static inline bool f8_wide(int64_t rows_a, int64_t rows_b) { return ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256) >= 192; }
-
-static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int type, int64_t ldc, hipStream_t s) {
-    return ddg_with_type(type, [&](auto t) {
-        using TO = decltype(t);
-        constexpr bool EXPAND = !std::is_same<TO, bf16_t>::value;
-        auto go = [&](auto mt, auto nt, auto wm, auto wn) {
-            constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
-            using S = F8Shape<MT, NT, WM, WN>;
-            F8Gemm g;
-            int rc = f8_problem<S>(a, b, bias, c, ldc, g);
-            const auto kernel = k_f8_gemm<MT, NT, WM, WN, EXPAND, TO>;
-            if (rc || (rc = f8_lds(kernel, S::LDS(sizeof(TO))))) return rc;
-            kernel<<<g.tiles_m * g.tiles_n, 64 * WM * WN, S::LDS(sizeof(TO)), s>>>(g);
-            DDG_CHECK_LAUNCH();
-            return (int)DDG_OK;
-        };
-        if constexpr (!EXPAND)
-            if (f8_wide(a.rows, b.rows)) return go(Int<8>(), Int<4>(), Int<2>(), Int<4>());
-        return go(Int<4>(), Int<4>(), Int<2>(), Int<2>());
-    });
+static F8Join f8_joined(const F8Operand &a, const F8Operand &b, const F8Split &sp, const float *parts, const float *bias, void *c,
+                        int64_t ldc) {
+    return {parts, a.rows, b.rows, (uint32_t)sp.splits, bias, c, ldc};
 }
-
-// dx = gy wt, dw = gyt xt
-static int f8_gemm_grads(const F8Operand &gy, const F8Operand &wt, void *dx, int dx_type, int64_t ld_dx, const F8Operand &gyt,
-                         const F8Operand &xt, float *dw, hipStream_t s) {
-    if (dx_type == DDG_BF16 && f8_wide(gy.rows, wt.rows)) {
-        const int rc = f8_gemm(gy, wt, nullptr, dx, dx_type, ld_dx, s);
-        return rc ? rc : f8_gemm(gyt, xt, nullptr, dw, DDG_F32, xt.rows, s);
-    }
-    return ddg_with_type(dx_type, [&](auto t) {
-        using TO = decltype(t);
-        using S = F8Shape<4, 4, 2, 2>;
-        F8Gemm gw, gx;
-        const auto kernel = k_f8_gemm_grads<!std::is_same<TO, bf16_t>::value, TO>;
-        int rc = f8_problem<S>(gyt, xt, nullptr, dw, xt.rows, gw);
-        if (rc || (rc = f8_problem<S>(gy, wt, nullptr, dx, ld_dx, gx)) || (rc = f8_lds(kernel, S::LDS(4)))) return rc;
-        kernel<<<gw.tiles_m * gw.tiles_n + gx.tiles_m * gx.tiles_n, 256, S::LDS(4), s>>>(gw, gx);
+static inline int64_t f8_join_grid(const F8Join &j) { return j.splits > 1 ? ceil_div64(j.M * ((j.N + 3) / 4), 256) : 0; }
+// whichever of the two was split (b: fp32)
+static int f8_join_parts(const F8Join &a, int type, const F8Join &b, hipStream_t s) {
+    const int64_t ga = f8_join_grid(a), gb = f8_join_grid(b);
+    if (ga + gb == 0) return DDG_OK;
+    if (ga + gb > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
+    return ddg_with_type(type, [&](auto t) {
+        k_f8_join<decltype(t)><<<(unsigned)(ga + gb), 256, 0, s>>>(a, (uint32_t)ga, b);
         DDG_CHECK_LAUNCH();
         return (int)DDG_OK;
     });
+}
+
+static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int type, int64_t ldc, float *parts, hipStream_t s) {
+    const F8Split sp = f8_split_one(a.rows, b.rows, a.cols, type == DDG_BF16);
+    const bool narrow = f8_stages(a.rows, b.rows, a.cols, 128) < 8 * F8_WORKGROUPS;
+    auto go = [&](auto mt, auto nt, auto wm, auto wn, auto expand, auto to) {
+        using TO = decltype(to);
+        constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+        using S = F8Shape<MT, NT, WM, WN>;
+        F8Gemm g;
+        int rc = f8_problem<S>(a, b, bias, c, ldc, sp, parts, g);
+        const auto kernel = k_f8_gemm<MT, NT, WM, WN, decltype(expand)::value, TO>;
+        if (rc || (rc = f8_lds(kernel, S::LDS(sizeof(TO))))) return rc;
+        kernel<<<g.tiles_m * g.tiles_n * g.splits, 64 * WM * WN, S::LDS(sizeof(TO)), s>>>(g);
+        DDG_CHECK_LAUNCH();
+        return (int)DDG_OK;
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    auto tiles = [&](auto expand, auto to) {
+        return narrow ? go(Int<4>(), Int<2>(), Int<2>(), Int<2>(), expand, to) : go(Int<4>(), Int<4>(), Int<2>(), Int<2>(), expand, to);
+    };
+    int rc;
+    if (sp.splits > 1) rc = type == DDG_BF16 ? tiles(no, float()) : tiles(yes, float());
+    else if (type == DDG_BF16 && f8_wide(a.rows, b.rows)) rc = go(Int<8>(), Int<4>(), Int<2>(), Int<4>(), no, bf16_t());
+    else rc = type == DDG_BF16 ? tiles(no, bf16_t()) : type == DDG_F16 ? tiles(yes, f16_t()) : tiles(yes, float());
+    return rc ? rc : f8_join_parts(f8_joined(a, b, sp, parts, bias, c, ldc), type, F8Join{nullptr, 0, 0, 1, nullptr, nullptr, 0}, s);
+}
+
+// the gradients' products: dx [rows, in] over out, dw [out, in] over rows
+struct F8GradSplits {
+    bool apart, narrow;                 // two launches (dx in 256 x 256 tiles); 128 x 64 tiles
+    F8Split dx, dw;
+};
+static inline F8GradSplits f8_grad_splits(int64_t rows, int64_t out, int64_t in, bool bf16) {
+    F8GradSplits g;
+    g.apart = bf16 && f8_wide(rows, in);
+    g.narrow = f8_stages(rows, in, out, 128) + f8_stages(out, in, rows, 128) < 8 * F8_WORKGROUPS;
+    const int bn = g.narrow ? 64 : 128;
+    const int64_t all = f8_stages(rows, in, out, bn) + f8_stages(out, in, rows, bn);
+    g.dx = g.apart ? f8_split_one(rows, in, out, bf16) : f8_split(rows, in, out, all);
+    g.dw = g.apart ? f8_split_one(out, in, rows, false) : f8_split(out, in, rows, all);
+    return g;
+}
+// dx = gy wt, dw = gyt xt
+static int f8_gemm_grads(const F8Operand &gy, const F8Operand &wt, void *dx, int dx_type, int64_t ld_dx, float *parts_dx,
+                         const F8Operand &gyt, const F8Operand &xt, float *dw, float *parts_dw, hipStream_t s) {
+    const F8GradSplits sp = f8_grad_splits(gy.rows, gy.cols, wt.rows, dx_type == DDG_BF16);
+    if (sp.apart) {
+        const int rc = f8_gemm(gy, wt, nullptr, dx, dx_type, ld_dx, parts_dx, s);
+        return rc ? rc : f8_gemm(gyt, xt, nullptr, dw, DDG_F32, xt.rows, parts_dw, s);
+    }
+    auto go = [&](auto nt, auto expand, auto to) {
+        using S = F8Shape<4, decltype(nt)::value, 2, 2>;
+        F8Gemm gw, gx;
+        const auto kernel = k_f8_gemm_grads<decltype(nt)::value, decltype(expand)::value, decltype(to)>;
+        int rc = f8_problem<S>(gyt, xt, nullptr, dw, xt.rows, sp.dw, parts_dw, gw);
+        if (rc || (rc = f8_problem<S>(gy, wt, nullptr, dx, ld_dx, sp.dx, parts_dx, gx)) || (rc = f8_lds(kernel, S::LDS(4)))) return rc;
+        kernel<<<gw.tiles_m * gw.tiles_n * gw.splits + gx.tiles_m * gx.tiles_n * gx.splits, 256, S::LDS(4), s>>>(gw, gx);
+        DDG_CHECK_LAUNCH();
+        return (int)DDG_OK;
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    auto tiles = [&](auto expand, auto to) { return sp.narrow ? go(Int<2>(), expand, to) : go(Int<4>(), expand, to); };
+    int rc;
+    if (sp.dx.splits > 1) rc = dx_type == DDG_BF16 ? tiles(no, float()) : tiles(yes, float());
+    else rc = dx_type == DDG_BF16 ? tiles(no, bf16_t()) : dx_type == DDG_F16 ? tiles(yes, f16_t()) : tiles(yes, float());
+    return rc ? rc : f8_join_parts(f8_joined(gy, wt, sp.dx, parts_dx, nullptr, dx, ld_dx), dx_type,
+                                   f8_joined(gyt, xt, sp.dw, parts_dw, nullptr, dw, xt.rows), s);
 }
 
 extern "C" int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t out, int64_t in, void *packed, void *packed_t,
@@ -668,9 +777,11 @@ extern "C" int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t 
     });
 }
 
-extern "C" size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t in) {
-    if (!f8_dims_ok(rows, in) || in < 1) return 0;
-    return rows <= F8_SKINNY ? 0 : ddg_fp8_operand_bytes(rows, in);
+extern "C" size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t out, int64_t in) {
+    if (!f8_dims_ok(rows, in) || !f8_dims_ok(out, 0) || in < 1 || out < 1) return 0;
+    if (rows <= F8_SKINNY) return 0;
+    // (the result's type decides about 256 x 256 tiles, which are not split: room for either)
+    return ddg_fp8_operand_bytes(rows, in) + f8_parts_bytes(f8_split_one(rows, out, in, false), rows, out);
 }
 
 extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t rows, const void *packed_w, int64_t out, int64_t in,
@@ -705,16 +816,16 @@ extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t r
                 return nk > 8 ? go(Int<16>()) : go(Int<8>());
             });
         });
-    if (!workspace || workspace_bytes < ddg_fp8_linear_workspace_bytes(rows, in)) return DDG_E_WORKSPACE;
+    if (!workspace || workspace_bytes < ddg_fp8_linear_workspace_bytes(rows, out, in)) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 255) return DDG_E_ARG;
     const F8Operand a = f8_operand(workspace, rows, in);
     const int rc = f8_pack_rows(x, x_type, ld_x, a, s);
-    return rc ? rc : f8_gemm(a, w, bias, y, y_type, ld_y, s);
+    return rc ? rc : f8_gemm(a, w, bias, y, y_type, ld_y, (float *)((char *)workspace + ddg_fp8_operand_bytes(rows, in)), s);
 }
 
 struct F8GradWs {
     void *dy, *dyt, *xt;
-    float *sums;
+    float *sums, *parts_dx, *parts_dw;
     size_t bytes;
 };
 static inline F8GradWs f8_grad_carve(void *base, int64_t rows, int64_t out, int64_t in) {
@@ -730,6 +841,15 @@ static inline F8GradWs f8_grad_carve(void *base, int64_t rows, int64_t out, int6
     w.dyt = take(ddg_fp8_operand_bytes(out, rows));
     w.xt = take(ddg_fp8_operand_bytes(in, rows));
     w.sums = (float *)take((size_t)ceil_div64(rows, F8_BLOCK) * out * 4);
+    size_t px = 0, pw = 0;                              // (either way that dx's type may have them done)
+    for (int bf16 = 0; bf16 < 2; ++bf16) {
+        const F8GradSplits sp = f8_grad_splits(rows, out, in, bf16);
+        const size_t x = f8_parts_bytes(sp.dx, rows, in), y = f8_parts_bytes(sp.dw, out, in);
+        px = x > px ? x : px;
+        pw = y > pw ? y : pw;
+    }
+    w.parts_dx = (float *)take(px);
+    w.parts_dw = (float *)take(pw);
     w.bytes = o;
     return w;
 }
@@ -769,5 +889,5 @@ extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, 
         k_f8_colsum<<<(unsigned)ceil_div64(out, 64), 256, 0, s>>>(w.sums, row_tiles, out, db);
         DDG_CHECK_LAUNCH();
     }
-    return f8_gemm_grads(gy, f8_operand((void *)packed_wt, in, out), dx, dx_type, ld_dx, gyt, xt, dw, s);
+    return f8_gemm_grads(gy, f8_operand((void *)packed_wt, in, out), dx, dx_type, ld_dx, w.parts_dx, gyt, xt, dw, w.parts_dw, s);
 }

@@ -840,7 +840,7 @@ def linear_fp8(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype]
         op, ldo = _matrix(out, "out")
     dev = x.get_device()
     stream = _on(dev, weight.packed, bias, out)
-    nb = _bytes("ddg_fp8_linear_workspace_bytes", rows, inn)
+    nb = _bytes("ddg_fp8_linear_workspace_bytes", rows, outd, inn)
     ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
     _call(dev, lib().ddg_fp8_linear, "ddg_fp8_linear", xp, _type(x, "x"), ld, rows, weight.packed.data_ptr(), outd, inn,
           _ptr(bias, torch.float32), op, _type(out, "out"), ldo, ws.data_ptr() if nb else None, nb, stream)

@@ -602,7 +602,7 @@ int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, int state_bit
 size_t ddg_fp8_operand_bytes(int64_t rows, int64_t cols);
 int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t out, int64_t in, void *packed, void *packed_t,
                         void *stream);
-size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t in);
+size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t out, int64_t in);
 int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t rows, const void *packed_w, int64_t out, int64_t in,
                    const float *bias, void *y, int y_type, int64_t ld_y, void *workspace, size_t workspace_bytes,
                    void *stream);

@@ -110,7 +110,7 @@ def test_fp8_grads_refuse(kw, rc):
 def test_workspace_sizes_of_bad_shapes():
     L = _lib.lib()
     assert L.ddg_embedding_grad_workspace_bytes(-1, 4) == 0 and L.ddg_embedding_grad_workspace_bytes(4, 0) == 0
-    assert L.ddg_fp8_operand_bytes(-1, 4) == 0 and L.ddg_fp8_linear_workspace_bytes(4, 0) == 0
+    assert L.ddg_fp8_operand_bytes(-1, 4) == 0 and L.ddg_fp8_linear_workspace_bytes(4, 4, 0) == 0
     assert L.ddg_fp8_linear_grads_workspace_bytes(4, 0, 4) == 0
     assert L.ddg_adamw_workspace_bytes(None, 3) == 0
 
