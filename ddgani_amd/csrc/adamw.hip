@@ -170,15 +170,15 @@ __device__ __forceinline__ void decode(uint32_t w, float scale, float (&y)[ADW_V
     y[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * scale;
     y[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * scale;
 }
-__device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int n) {
-    if (n >= ADW_VEC) return *(const uint32_t *)p;
+template <bool STREAM> __device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int n) {
+    if (n >= ADW_VEC) return STREAM ? __builtin_nontemporal_load((const uint32_t *)p) : *(const uint32_t *)p;
     uint32_t w = 0;
     for (int i = 0; i < n; ++i) w |= (uint32_t)p[i] << (8 * i);
     return w;
 }
-__device__ __forceinline__ void store_codes(uint8_t *p, int n, uint32_t w) {
-    if (n >= ADW_VEC)
-        *(uint32_t *)p = w;
+template <bool STREAM> __device__ __forceinline__ void store_codes(uint8_t *p, int n, uint32_t w) {
+    if (n >= ADW_VEC && STREAM) __builtin_nontemporal_store(w, (uint32_t *)p);
+    else if (n >= ADW_VEC) *(uint32_t *)p = w;
     else
         for (int i = 0; i < n; ++i) p[i] = (uint8_t)(w >> (8 * i));
 }
@@ -190,7 +190,8 @@ struct AdwState {
 
 // A wave owns UNITS blocks of 256 elements, four consecutive elements per lane: every access is one contiguous piece per
 // wave, and a block's maximum is one reduction over the wave.  All loads come first.  Workgroups take the table from its end:
-// what the norm read last is still in the 256 MB cache.  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
+// what the norm read last is still in the 256 MB cache, and in the wide variant everything but the gradients goes past it
+// (332 million elements 1 185 -> STREAMUS us).  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
 // adds up the partial norms and forms the step's scalars itself, which is quicker than a launch of its own for them.
 // (One launch for norm and step, whose last workgroup to arrive goes on alone, is slower: an atomic that all XCDs share takes
 // 85 ns a workgroup.)
@@ -199,6 +200,7 @@ struct AdwState {
 template <class P, class G, bool BITS8, bool MASTER, int UNITS, bool SELF>
 __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, AdwControl *ctl, AdwHyper h, float one_m_b1, float b2,
                                                   float one_m_b2, float eps, const double *__restrict__ part, int parts) {
+    constexpr bool WIDE = UNITS > 1;
     const int chunk = (int)(gridDim.x - 1 - blockIdx.x);
     const AdwEntry &e = tb.t[adw_find(tb, chunk)];
     P *__restrict__ const p = (P *)e.p;
@@ -212,17 +214,17 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, AdwC
         const int64_t b = base + u * ADW_BLOCK, i = b + lane * ADW_VEC, f = e.off + i;
         const int n = e.n - i >= ADW_VEC ? ADW_VEC : e.n > i ? (int)(e.n - i) : 0;
         load_n<ADW_VEC>(g + i, n, gv[u]);
-        if (MASTER) load_n<ADW_VEC>(st.master + f, n, wv[u]);
-        else load_n<ADW_VEC>(p + i, n, wv[u]);
+        if (MASTER) load_n<ADW_VEC, WIDE>(st.master + f, n, wv[u]);
+        else load_n<ADW_VEC, WIDE>(p + i, n, wv[u]);
         if (BITS8) {
-            mc[u] = load_codes((const uint8_t *)st.m + f, n);
-            vc[u] = load_codes((const uint8_t *)st.v + f, n);
+            mc[u] = load_codes<WIDE>((const uint8_t *)st.m + f, n);
+            vc[u] = load_codes<WIDE>((const uint8_t *)st.v + f, n);
             const int64_t blk = (e.off + b) / ADW_BLOCK;
             ms[u] = b < e.n ? st.ms[blk] : 0.f;
             vs[u] = b < e.n ? st.vs[blk] : 0.f;
         } else {
-            load_n<ADW_VEC>((const float *)st.m + f, n, mv[u]);
-            load_n<ADW_VEC>((const float *)st.v + f, n, vv[u]);
+            load_n<ADW_VEC, WIDE>((const float *)st.m + f, n, mv[u]);
+            load_n<ADW_VEC, WIDE>((const float *)st.v + f, n, vv[u]);
         }
     }
     AdwScalars sc;
@@ -272,8 +274,8 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, AdwC
                 top_r = fmaxf(top_r, r[k]);
             }
         }
-        if (MASTER) store_n<ADW_VEC>(st.master + f, n, w);
-        store_n<ADW_VEC>(p + i, n, w);
+        if (MASTER) store_n<ADW_VEC, WIDE>(st.master + f, n, w);
+        store_n<ADW_VEC, WIDE>(p + i, n, w);
         if (BITS8) {
             const int64_t blk = (e.off + b) / ADW_BLOCK;
             top_m = wave_max(top_m);
@@ -284,15 +286,15 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, AdwC
                 m[k] = m[k] * im;
                 r[k] = r[k] * ir;
             }
-            store_codes((uint8_t *)st.m + f, n, encode_nearest(m));
-            store_codes((uint8_t *)st.v + f, n, encode_dithered(r, (uint32_t)f, sc.dither));
+            store_codes<WIDE>((uint8_t *)st.m + f, n, encode_nearest(m));
+            store_codes<WIDE>((uint8_t *)st.v + f, n, encode_dithered(r, (uint32_t)f, sc.dither));
             if (lane == 0) {
                 st.ms[blk] = top_m >= ADW_TINY ? top_m * (1.f / 448.f) : 0.f;
                 st.vs[blk] = top_r >= ADW_TINY ? top_r * (1.f / 448.f) : 0.f;
             }
         } else {
-            store_n<ADW_VEC>((float *)st.m + f, n, m);
-            store_n<ADW_VEC>((float *)st.v + f, n, v);
+            store_n<ADW_VEC, WIDE>((float *)st.m + f, n, m);
+            store_n<ADW_VEC, WIDE>((float *)st.v + f, n, v);
         }
     }
 }

@@ -14,6 +14,7 @@
 #include "types.h"
 
 #define EMB_NT 256
+#define EMB_STREAM (16 << 20)         // elements of a gradient from which it is stored past the caches (2 % less time at 262 million)
 #define EMB_VEC 8                     // elements per thread and row: 16 bytes of a 16-bit type
 
 // A lane's eight columns of rows of D: [at, at + 8) is what it loads, always whole and inside the row, so that no load sits
@@ -33,16 +34,14 @@ template <bool TINY, class T> __device__ __forceinline__ vec8<T> load_row(const 
     }
     return v;
 }
-template <bool TINY, class T> __device__ __forceinline__ void store_row(T *row, const Columns &c, const float (&v)[EMB_VEC]) {
-    vec8<T> o;
-#pragma unroll
-    for (int i = 0; i < EMB_VEC; ++i) o[i] = (T)v[i];
+template <bool TINY, bool STREAM = false, class T>
+__device__ __forceinline__ void store_row(T *row, const Columns &c, const float (&v)[EMB_VEC]) {
     if (!TINY && c.col == c.at) {
-        __builtin_memcpy(row + c.at, &o, sizeof(o));
+        store_n<EMB_VEC, STREAM>(row + c.at, EMB_VEC, v);
     } else {
 #pragma unroll
         for (int i = 0; i < EMB_VEC; ++i)
-            if (c.at + i >= c.col && c.at + i < c.D) row[c.at + i] = o[i];
+            if (c.at + i >= c.col && c.at + i < c.D) row[c.at + i] = (T)v[i];
     }
 }
 template <class T> __device__ __forceinline__ void add_row(float (&acc)[EMB_VEC], const vec8<T> &v) {
@@ -55,7 +54,8 @@ template <class ID> __device__ __forceinline__ uint32_t emb_key(const ID *ids, i
     return (uint64_t)v < (uint64_t)V && v != padding_idx ? (uint32_t)v : (uint32_t)V;      // V: no row
 }
 
-// U rows per thread group: their id loads, then their row loads, are in flight together
+// U rows per thread group: their id loads, then their row loads, are in flight together.  Large results (U > 1) are stored past
+// the caches: 65 488 rows of 1 024 fp32 -> bf16 50.6 us with ordinary stores, 42.0 us so.
 template <class TI, class TO, class ID, int U, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embed(const ID *__restrict__ ids, int64_t n, const TI *__restrict__ table, int64_t V,
                                                   int D, int64_t ld, float scale, TO *__restrict__ out, int64_t ldo, int lg_tpr) {
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(EMB_NT) void k_embed(const ID *__restrict__ ids, in
         float f[EMB_VEC];
 #pragma unroll
         for (int i = 0; i < EMB_VEC; ++i) f[i] = (uint64_t)id[u] < (uint64_t)V ? (float)v[u][i] * scale : 0.f;
-        store_row<TINY>(out + r * ldo, c, f);
+        store_row<TINY, (U > 1)>(out + r * ldo, c, f);
     }
 }
 
@@ -391,7 +391,7 @@ template <class T, class TO, bool TINY>
 __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n,
                                                       int64_t V, const T *__restrict__ dy, int64_t ld, int D,
                                                       const float *__restrict__ part1, const float *__restrict__ part2, float scale,
-                                                      int accumulate, TO *__restrict__ out, int64_t ldo, int lg, int rows, int slabs) {
+                                                      int accumulate, TO *__restrict__ out, int64_t ldo, int lg, int rows, int slabs, int stream) {
     const uint32_t rblock = blockIdx.x / slabs, slab = blockIdx.x - rblock * slabs;
     const int lane = threadIdx.x & 63, lanes = 1 << lg, in_group = lane & (lanes - 1), group = lane >> lg;
     const int64_t wave0 = ((int64_t)rblock * (EMB_NT / 64) + (threadIdx.x >> 6)) * ((64 >> lg) * rows);
@@ -439,7 +439,8 @@ __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(co
             if (accumulate) old = load_row<TINY>(o, c);
 #pragma unroll
             for (int i = 0; i < EMB_VEC; ++i) acc[i] = (float)old[i] + scale * acc[i];
-            store_row<TINY>(o, c, acc);
+            if (stream) store_row<TINY, true>(o, c, acc);
+            else store_row<TINY>(o, c, acc);
         }
 #pragma unroll
         for (int i = 0; i < EMB_VEC; ++i) acc[i] = 0.f;
@@ -575,7 +576,7 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
                 using TO = decltype(to);
                 k_embg_rows<TI, TO, TINY><<<(unsigned)(rgrid * rslabs), EMB_NT, 0, s>>>(
                     w.key[cur], w.pos[cur], n, V, (const TI *)dy, ld_dy, D, w.part1, w.part2, scale, accumulate, (TO *)out, ld_out,
-                    rlg, (int)rows, (int)rslabs);
+                    rlg, (int)rows, (int)rslabs, V * D > EMB_STREAM);
                 DDG_CHECK_LAUNCH();
                 return (int)DDG_OK;
             });

@@ -18,13 +18,21 @@ template <class F> static inline int ddg_with_type(int t, F &&f) {
     }
 }
 
-// n <= N consecutive elements -> fp32 (elements from n on read as 0).  A full vector is moved with the widest loads; the
+// a 16-byte store past the caches, at any alignment
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ void store16_streaming(void *p, const void *v) {
+    i32x4_any w;
+    __builtin_memcpy(&w, v, 16);
+    __builtin_nontemporal_store(w, (i32x4_any *)p);
+}
+
+// n <= N consecutive elements -> fp32 (elements from n on read as 0).  A full vector is moved with the widest access; the
 // address needs the alignment of one element only (gfx950 serves unaligned 16-byte accesses of global memory), so rows of
-// odd length take the same path.
-template <int N, class T> __device__ __forceinline__ void load_n(const T *p, int n, float (&v)[N]) {
+// odd length take the same path.  STREAM: past the caches, for what is larger than they are and touched once.
+template <int N, bool STREAM = false, class T> __device__ __forceinline__ void load_n(const T *p, int n, float (&v)[N]) {
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
     if (n >= N) {
-        T t[N];
-        __builtin_memcpy(t, p, sizeof(t));
+        const vec t = STREAM ? __builtin_nontemporal_load((const vec *)p) : *(const vec *)p;
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = (float)t[i];
     } else {
@@ -32,12 +40,14 @@ template <int N, class T> __device__ __forceinline__ void load_n(const T *p, int
         for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
     }
 }
-template <int N, class T> __device__ __forceinline__ void store_n(T *p, int n, const float (&v)[N]) {
+template <int N, bool STREAM = false, class T> __device__ __forceinline__ void store_n(T *p, int n, const float (&v)[N]) {
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
     if (n >= N) {
-        T t[N];
+        vec t;
 #pragma unroll
         for (int i = 0; i < N; ++i) t[i] = (T)v[i];
-        __builtin_memcpy(p, t, sizeof(t));
+        if (STREAM) __builtin_nontemporal_store(t, (vec *)p);
+        else *(vec *)p = t;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
