@@ -24,13 +24,13 @@ struct Columns {
     int col, at, D;
     __device__ Columns(int c, int d) : col(c), at(c < d - EMB_VEC ? c : d > EMB_VEC ? d - EMB_VEC : 0), D(d) {}
 };
-template <bool TINY, class T> __device__ __forceinline__ vec8<T> load_row(const T *row, const Columns &c) {
+template <bool TINY, bool STREAM = false, class T> __device__ __forceinline__ vec8<T> load_row(const T *row, const Columns &c) {
     vec8<T> v;
     if (TINY) {
 #pragma unroll
         for (int i = 0; i < EMB_VEC; ++i) v[i] = i < c.D ? row[i] : (T)0.f;
     } else {
-        v = load_whole(row + c.at);
+        v = load_whole<STREAM>(row + c.at);
     }
     return v;
 }
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict
     for (int j = 0; j < 64; j += 8) {                   // eight rows in flight, and with them the next eight positions
         vec8<T> v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = load_row<TINY>(src + (int64_t)p[u] * ld, cs);
+        for (int u = 0; u < 8; ++u) v[u] = load_row<TINY, true>(src + (int64_t)p[u] * ld, cs);
         const int next = j + 8 < 64 ? j + 8 : j;
 #pragma unroll
         for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * 64 + next + u] : (uint32_t)(c * 64 + next + u);
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(co
     auto fetch = [&](int j, vec8<T>(&w)[4]) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)                     // (behind the list: token 0, not used)
-            w[u] = load_row<TINY>(dy + (int64_t)__shfl(item_pos, j + u, lanes) * ld, c);
+            w[u] = load_row<TINY, true>(dy + (int64_t)__shfl(item_pos, j + u, lanes) * ld, c);
     };
     for (int base = 0; base < total; base += lanes) {
         // lane l: item base + l of the list, its row by counting the rows that end before it

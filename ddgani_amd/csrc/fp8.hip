@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void k_f8_pack_rows(const T *__restrict__ x, i
     if (g >= rows * nb) return;                         // (whole DPP rows leave together)
     const int64_t r = g / nb, b = g - r * nb, c = b * F8_BLOCK + (threadIdx.x & 15) * 8;
     float v[8], a = 0.f;
-    load_n<8>(x + r * ld + c, cols - c >= 8 ? 8 : cols > c ? (int)(cols - c) : 0, v);
+    load_n<8, true>(x + r * ld + c, cols - c >= 8 ? 8 : cols > c ? (int)(cols - c) : 0, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[i]));
     const int e = f8_exponent(row16_max(a));

@@ -57,10 +57,9 @@ template <int N, bool STREAM = false, class T> __device__ __forceinline__ void s
 
 // eight consecutive elements, all of them in bounds: one load without a branch around it
 template <class T> using vec8 = T __attribute__((ext_vector_type(8)));
-template <class T> __device__ __forceinline__ vec8<T> load_whole(const T *p) {
-    vec8<T> v;
-    __builtin_memcpy(&v, p, sizeof(v));
-    return v;
+template <bool STREAM = false, class T> __device__ __forceinline__ vec8<T> load_whole(const T *p) {
+    typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    return STREAM ? __builtin_nontemporal_load((const vec *)p) : *(const vec *)p;
 }
 
 // maximum over the 16 lanes of a DPP row, in every lane
