@@ -207,19 +207,27 @@ template <class T> __global__ __launch_bounds__(256) void k_f8_pack_grads(F8Pack
     else f8_pack_one<T, F8_COLS>(x, blockIdx.x - tiles_dy);
 }
 
-// column sums from those of the row tiles: 64 columns per workgroup, its four waves share the tiles
-__global__ __launch_bounds__(256) void k_f8_colsum(const float *__restrict__ part, int64_t tiles, int64_t cols, float *__restrict__ out) {
-    __shared__ float w[4][64];
+// column sums from those of the row tiles: 64 columns per workgroup, its four waves share the tiles (lds: 1 KB)
+struct F8Colsum {
+    const float *part;
+    int64_t tiles, cols;
+    float *out;
+};
+__device__ __forceinline__ void f8_colsum(const F8Colsum &s, uint32_t block, float *lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t c = (int64_t)block * 64 + lane;
     float a = 0.f;
-    if (c < cols) {
+    if (c < s.cols) {
 #pragma unroll 8
-        for (int64_t t = wave; t < tiles; t += 4) a += part[t * cols + c];
+        for (int64_t t = wave; t < s.tiles; t += 4) a += s.part[t * s.cols + c];
     }
-    w[wave][lane] = a;
+    lds[wave * 64 + lane] = a;
     __syncthreads();
-    if (wave == 0 && c < cols) out[c] = (w[0][lane] + w[1][lane]) + (w[2][lane] + w[3][lane]);
+    if (wave == 0 && c < s.cols) s.out[c] = (lds[lane] + lds[64 + lane]) + (lds[128 + lane] + lds[192 + lane]);
+}
+__global__ __launch_bounds__(256) void k_f8_colsum(F8Colsum s) {
+    __shared__ float lds[256];
+    f8_colsum(s, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -466,11 +474,15 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO>
 __global__ __launch_bounds__(64 * WM * WN, MT * NT <= 8 ? 3 : 2) void k_f8_gemm(F8Gemm g) {
     f8_gemm_tile<MT, NT, WM, WN, EXPAND, TO>(g, blockIdx.x);
 }
-// dW (fp32) and dX of one layer in one launch: neither has the tiles for whole rounds of the CUs.  dW's, the longer ones, first
-template <int NT, bool EXPAND, class TO> __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void k_f8_gemm_grads(F8Gemm dw, F8Gemm dx) {
-    const uint32_t first = dw.tiles_m * dw.tiles_n * dw.splits;
-    if (blockIdx.x < first) f8_gemm_tile<4, NT, 2, 2, true, float>(dw, blockIdx.x);
-    else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, blockIdx.x - first);
+// dW (fp32) and dX of one layer, and db, in one launch: neither product has the tiles for whole rounds of the CUs.  db's
+// workgroups (`sums`, may be none) first, then dW's, the longer ones
+template <int NT, bool EXPAND, class TO>
+__global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void k_f8_gemm_grads(F8Gemm dw, F8Gemm dx, F8Colsum db, uint32_t sums) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const uint32_t first = dw.tiles_m * dw.tiles_n * dw.splits, id = blockIdx.x - sums;
+    if (blockIdx.x < sums) f8_colsum(db, blockIdx.x, (float *)lds);
+    else if (id < first) f8_gemm_tile<4, NT, 2, 2, true, float>(dw, id);
+    else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, id - first);
 }
 
 // C = bias + sum of the parts, in their order; four columns per thread
@@ -671,7 +683,8 @@ static int f8_problem(const F8Operand &a, const F8Operand &b, const float *bias,
          split ? b.rows : ldc, (uint32_t)tm, (uint32_t)tn, (uint32_t)sp.splits, (uint32_t)sp.blocks};
     return DDG_OK;
 }
-template <class K> static int f8_lds(K kernel, int bytes) {
+template <class K> static int f8_lds(K kernel, int bytes) {        // more than 64 KB has to be asked for
+    if (bytes <= 65536) return DDG_OK;
     return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? DDG_OK
                                                                                                                  : DDG_E_LAUNCH;
 }
@@ -736,9 +749,14 @@ static inline F8GradSplits f8_grad_splits(int64_t rows, int64_t out, int64_t in,
 }
 // dx = gy wt, dw = gyt xt
 static int f8_gemm_grads(const F8Operand &gy, const F8Operand &wt, void *dx, int dx_type, int64_t ld_dx, float *parts_dx,
-                         const F8Operand &gyt, const F8Operand &xt, float *dw, float *parts_dw, hipStream_t s) {
+                         const F8Operand &gyt, const F8Operand &xt, float *dw, float *parts_dw, const F8Colsum &db, hipStream_t s) {
     const F8GradSplits sp = f8_grad_splits(gy.rows, gy.cols, wt.rows, dx_type == DDG_BF16);
+    const uint32_t sums = db.out ? (uint32_t)ceil_div64(db.cols, 64) : 0;
     if (sp.apart) {
+        if (sums) {
+            k_f8_colsum<<<sums, 256, 0, s>>>(db);
+            DDG_CHECK_LAUNCH();
+        }
         const int rc = f8_gemm(gy, wt, nullptr, dx, dx_type, ld_dx, parts_dx, s);
         return rc ? rc : f8_gemm(gyt, xt, nullptr, dw, DDG_F32, xt.rows, parts_dw, s);
     }
@@ -748,7 +766,7 @@ static int f8_gemm_grads(const F8Operand &gy, const F8Operand &wt, void *dx, int
         const auto kernel = k_f8_gemm_grads<decltype(nt)::value, decltype(expand)::value, decltype(to)>;
         int rc = f8_problem<S>(gyt, xt, nullptr, dw, xt.rows, sp.dw, parts_dw, gw);
         if (rc || (rc = f8_problem<S>(gy, wt, nullptr, dx, ld_dx, sp.dx, parts_dx, gx)) || (rc = f8_lds(kernel, S::LDS(4)))) return rc;
-        kernel<<<gw.tiles_m * gw.tiles_n * gw.splits + gx.tiles_m * gx.tiles_n * gx.splits, 256, S::LDS(4), s>>>(gw, gx);
+        kernel<<<sums + gw.tiles_m * gw.tiles_n * gw.splits + gx.tiles_m * gx.tiles_n * gx.splits, 256, S::LDS(4), s>>>(gw, gx, db, sums);
         DDG_CHECK_LAUNCH();
         return (int)DDG_OK;
     };
@@ -887,9 +905,6 @@ extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, 
     int rc = pack(dy_type, tiles_dy, x_type == dy_type ? tiles_x : 0);
     if (!rc && x_type != dy_type) rc = pack(x_type, 0, tiles_x);
     if (rc) return rc;
-    if (db && row_tiles > 1) {
-        k_f8_colsum<<<(unsigned)ceil_div64(out, 64), 256, 0, s>>>(w.sums, row_tiles, out, db);
-        DDG_CHECK_LAUNCH();
-    }
-    return f8_gemm_grads(gy, f8_operand((void *)packed_wt, in, out), dx, dx_type, ld_dx, w.parts_dx, gyt, xt, dw, w.parts_dw, s);
+    const F8Colsum sum = {w.sums, row_tiles, out, db && row_tiles > 1 ? db : nullptr};
+    return f8_gemm_grads(gy, f8_operand((void *)packed_wt, in, out), dx, dx_type, ld_dx, w.parts_dx, gyt, xt, dw, w.parts_dw, sum, s);
 }
