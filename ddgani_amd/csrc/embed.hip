@@ -14,6 +14,7 @@
 #include "types.h"
 
 #define EMB_NT 256
+#define EMB_MAX_D (1 << 26)           // columns are counted in 32 bits, slabs of them by the grid's second dimension
 #define EMB_STREAM (16 << 20)         // elements of a gradient from which it is stored past the caches (2 % less time at 262 million)
 #define EMB_VEC 8                     // elements per thread and row: 16 bytes of a 16-bit type
 
@@ -88,7 +89,7 @@ static inline int emb_lg_tpr(int D) {          // lanes per row: the power of tw
 
 extern "C" int ddg_embedding(const void *ids, int ids_64, int64_t n, const void *table, int table_type, int64_t V, int D,
                              int64_t ld_table, float scale, void *out, int out_type, int64_t ld_out, void *stream) {
-    if (n < 0 || V < 1 || V > 0x7FFFFFFF || D < 1 || ld_table < D || ld_out < D || !ddg_type_ok(table_type) ||
+    if (n < 0 || V < 1 || V > 0x7FFFFFFF || D < 1 || D > EMB_MAX_D || ld_table < D || ld_out < D || !ddg_type_ok(table_type) ||
         !ddg_type_ok(out_type) || (ids_64 != 0 && ids_64 != 1))
         return DDG_E_ARG;
     if (n == 0) return DDG_OK;
@@ -98,7 +99,7 @@ extern "C" int ddg_embedding(const void *ids, int ids_64, int64_t n, const void 
     // four rows per thread once that still leaves two workgroups per CU; one row below (few rows: latency, not bandwidth)
     const bool wide = ceil_div64(n, 4 * rpb) * slabs >= 512;
     const int64_t gx = ceil_div64(n, wide ? 4 * rpb : rpb);
-    if (gx > 0x7FFFFFFF || slabs > 65535) return DDG_E_UNSUPPORTED;
+    if (gx > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
     return ddg_with_type(table_type, [&](auto ti) {
         return ddg_with_type(out_type, [&](auto to) {
             using TI = decltype(ti);
@@ -511,14 +512,14 @@ static inline EmbWs emb_carve(void *base, int64_t n, int D) {
 }
 
 extern "C" size_t ddg_embedding_grad_workspace_bytes(int64_t n, int D) {
-    if (n < 0 || n > 0x7FFFFFFF || D < 1) return 0;
+    if (n < 0 || n > 0x7FFFFFFF || D < 1 || D > EMB_MAX_D) return 0;
     return emb_carve(nullptr, n, D).bytes;
 }
 
 extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const void *dy, int dy_type, int64_t ld_dy, int64_t V,
                                   int D, float scale, int64_t padding_idx, int accumulate, void *out, int out_type, int64_t ld_out,
                                   void *workspace, size_t workspace_bytes, void *stream) {
-    if (n < 0 || V < 1 || D < 1 || ld_dy < D || ld_out < D || !ddg_type_ok(dy_type) || !ddg_type_ok(out_type) ||
+    if (n < 0 || V < 1 || D < 1 || D > EMB_MAX_D || ld_dy < D || ld_out < D || !ddg_type_ok(dy_type) || !ddg_type_ok(out_type) ||
         (ids_64 != 0 && ids_64 != 1) || !out)
         return DDG_E_ARG;
     if (n > 0x7FFFFFFF || V > 0x7FFFFFFE) return DDG_E_UNSUPPORTED;
@@ -526,6 +527,16 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
     if (n > 0 && (!ids || !dy)) return DDG_E_ARG;
     if (!workspace || workspace_bytes < ddg_embedding_grad_workspace_bytes(n, D)) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 15) return DDG_E_ARG;
+    const int lg = emb_lg_tpr(D), rpb = EMB_NT >> lg;
+    const int slabs = (D + (EMB_VEC << lg) - 1) / (EMB_VEC << lg);
+    // k_embg_rows: groups of 8 to 64 lanes, and as many rows per group (16 at most, 32 per wave) as leave about 8 192 waves
+    const int rlg = lg < 3 ? 3 : lg > 6 ? 6 : lg, groups = 64 >> rlg;
+    const int64_t rslabs = ceil_div64(D, EMB_VEC << rlg);
+    int64_t rows = V * rslabs / ((int64_t)groups * 8192);
+    const int most = ROWS_MAX / groups < 16 ? ROWS_MAX / groups : 16;
+    rows = rows < 1 ? 1 : rows > most ? most : rows;
+    const int64_t rgrid = ceil_div64(V, EMB_NT / 64 * groups * rows);
+    if (rgrid * rslabs > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
     const EmbWs w = emb_carve(workspace, n, D);
     const SortPlan sp = sort_plan(n > 0 ? n : 1, V);
     const hipStream_t s = (hipStream_t)stream;
@@ -550,17 +561,6 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
         if (ids_64) sort(int64_t()); else sort(int32_t());
         DDG_CHECK_LAUNCH();
     }
-    const int lg = emb_lg_tpr(D), rpb = EMB_NT >> lg;
-    const int slabs = (D + (EMB_VEC << lg) - 1) / (EMB_VEC << lg);
-    if (slabs > 65535) return DDG_E_UNSUPPORTED;
-    // k_embg_rows: groups of 8 to 64 lanes, and as many rows per group (16 at most, 32 per wave) as leave about 8 192 waves
-    const int rlg = lg < 3 ? 3 : lg > 6 ? 6 : lg, groups = 64 >> rlg;
-    const int64_t rslabs = ceil_div64(D, EMB_VEC << rlg);
-    int64_t rows = V * rslabs / ((int64_t)groups * 8192);
-    const int most = ROWS_MAX / groups < 16 ? ROWS_MAX / groups : 16;
-    rows = rows < 1 ? 1 : rows > most ? most : rows;
-    const int64_t rgrid = ceil_div64(V, EMB_NT / 64 * groups * rows);
-    if (rgrid * rslabs > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
     return ddg_with_type(dy_type, [&](auto ti) {
         using TI = decltype(ti);
         auto sums = [&](auto tiny) {

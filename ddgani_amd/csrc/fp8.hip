@@ -640,8 +640,13 @@ static int f8_pack_rows(const void *x, int type, int64_t ld, const F8Operand &o,
 }
 static inline int64_t f8_tiles(int64_t rows, int64_t cols) { return ceil_div64(rows, F8_BLOCK) * ceil_div64(cols, F8_BLOCK); }
 
-// reductions are addressed with 32-bit offsets within a workgroup's 256 rows
+#define F8_WORKGROUPS 512                               // two per CU
+// Reductions are addressed with 32-bit offsets within a workgroup's 256 rows; tiles are counted in 32 bits (with their splits:
+// only where there are fewer tiles than F8_WORKGROUPS).  Checked in front of an entry point's first launch.
 #define F8_MAX_REDUCTION ((int64_t)1 << 24)
+static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
+    return f8_pad(cols) < F8_MAX_REDUCTION && ceil_div64(rows_a, 128) <= 0x0FFFFFFF / ceil_div64(rows_b, 64);
+}
 
 // Tiles are 256 x 256 (bf16 results only) once there are three quarters of a CU's worth of them; else 128 x 128, or 128 x 64 while
 // all tiles together have fewer than eight stages for each of 512 workgroups: there the time is latency.  A tile whose reduction
@@ -649,7 +654,6 @@ static inline int64_t f8_tiles(int64_t rows, int64_t cols) { return ceil_div64(r
 // four stages at least), which are added afterwards, where that saves more (0.6 us a stage) than it costs (a launch, 3 us, and
 // the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 13.7 us, 128 x 4096 x 4096
 // 36 -> 24 us; 256 x 1000 x 8192 would go from 16 to 21 us and is left whole.
-#define F8_WORKGROUPS 512
 static inline bool f8_wide(int64_t rows_a, int64_t rows_b) { return ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256) >= 192; }
 static inline int64_t f8_stages(int64_t rows_a, int64_t rows_b, int64_t cols, int bn) {
     return ceil_div64(rows_a, 128) * ceil_div64(rows_b, bn) * (f8_pad(cols) / F8_BLOCK);
@@ -674,14 +678,12 @@ static inline size_t f8_parts_bytes(const F8Split &sp, int64_t m, int64_t n) {
 }
 
 template <class S>
-static int f8_problem(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int64_t ldc, const F8Split &sp, float *parts,
-                      F8Gemm &g) {
-    const int64_t tm = ceil_div64(a.rows, S::BM), tn = ceil_div64(b.rows, S::BN), kp = f8_pad(a.cols);
-    if (kp >= F8_MAX_REDUCTION || tm * tn * sp.splits > 0x0FFFFFFF) return DDG_E_UNSUPPORTED;
+static F8Gemm f8_problem(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int64_t ldc, const F8Split &sp,
+                         float *parts) {
     const bool split = sp.splits > 1;
-    g = {a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s, b.rows, kp, split ? nullptr : bias, split ? parts : c,
-         split ? b.rows : ldc, (uint32_t)tm, (uint32_t)tn, (uint32_t)sp.splits, (uint32_t)sp.blocks};
-    return DDG_OK;
+    return {a.q, (const uint32_t *)a.s, a.rows, b.q, (const uint32_t *)b.s, b.rows, f8_pad(a.cols), split ? nullptr : bias,
+            split ? parts : c, split ? b.rows : ldc, (uint32_t)ceil_div64(a.rows, S::BM), (uint32_t)ceil_div64(b.rows, S::BN),
+            (uint32_t)sp.splits, (uint32_t)sp.blocks};
 }
 template <class K> static int f8_lds(K kernel, int bytes) {        // more than 64 KB has to be asked for
     if (bytes <= 65536) return DDG_OK;
@@ -712,10 +714,10 @@ static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, vo
         using TO = decltype(to);
         constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
         using S = F8Shape<MT, NT, WM, WN>;
-        F8Gemm g;
-        int rc = f8_problem<S>(a, b, bias, c, ldc, sp, parts, g);
+        const F8Gemm g = f8_problem<S>(a, b, bias, c, ldc, sp, parts);
         const auto kernel = k_f8_gemm<MT, NT, WM, WN, decltype(expand)::value, TO>;
-        if (rc || (rc = f8_lds(kernel, S::LDS(sizeof(TO))))) return rc;
+        const int rc = f8_lds(kernel, S::LDS(sizeof(TO)));
+        if (rc) return rc;
         kernel<<<g.tiles_m * g.tiles_n * g.splits, 64 * WM * WN, S::LDS(sizeof(TO)), s>>>(g);
         DDG_CHECK_LAUNCH();
         return (int)DDG_OK;
@@ -762,10 +764,11 @@ static int f8_gemm_grads(const F8Operand &gy, const F8Operand &wt, void *dx, int
     }
     auto go = [&](auto nt, auto expand, auto to) {
         using S = F8Shape<4, decltype(nt)::value, 2, 2>;
-        F8Gemm gw, gx;
+        const F8Gemm gw = f8_problem<S>(gyt, xt, nullptr, dw, xt.rows, sp.dw, parts_dw);
+        const F8Gemm gx = f8_problem<S>(gy, wt, nullptr, dx, ld_dx, sp.dx, parts_dx);
         const auto kernel = k_f8_gemm_grads<decltype(nt)::value, decltype(expand)::value, decltype(to)>;
-        int rc = f8_problem<S>(gyt, xt, nullptr, dw, xt.rows, sp.dw, parts_dw, gw);
-        if (rc || (rc = f8_problem<S>(gy, wt, nullptr, dx, ld_dx, sp.dx, parts_dx, gx)) || (rc = f8_lds(kernel, S::LDS(4)))) return rc;
+        const int rc = f8_lds(kernel, S::LDS(4));
+        if (rc) return rc;
         kernel<<<sums + gw.tiles_m * gw.tiles_n * gw.splits + gx.tiles_m * gx.tiles_n * gx.splits, 256, S::LDS(4), s>>>(gw, gx, db, sums);
         DDG_CHECK_LAUNCH();
         return (int)DDG_OK;
@@ -812,6 +815,7 @@ extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t r
         return DDG_E_ARG;
     if (rows == 0) return DDG_OK;
     if (!x || !y) return DDG_E_ARG;
+    if (!f8_product_ok(rows, out, in)) return DDG_E_UNSUPPORTED;
     const F8Operand w = f8_operand((void *)packed_w, out, in);
     const hipStream_t s = (hipStream_t)stream;
     if (rows <= F8_SKINNY)
@@ -885,6 +889,7 @@ extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, 
         !ddg_type_ok(dy_type) || !ddg_type_ok(x_type) || !ddg_type_ok(dx_type) || !dy || !x || !packed_wt || !dx || !dw ||
         ((uintptr_t)packed_wt & 255))
         return DDG_E_ARG;
+    if (!f8_product_ok(rows, in, out) || !f8_product_ok(out, in, rows)) return DDG_E_UNSUPPORTED;
     if (!workspace || workspace_bytes < ddg_fp8_linear_grads_workspace_bytes(rows, out, in)) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 255) return DDG_E_ARG;
     const F8GradWs w = f8_grad_carve(workspace, rows, out, in);

@@ -542,7 +542,7 @@ int ddg_decode_table(const float *code, const uint8_t *m, const double *obs, con
  * independent of each other; ld_*: elements between rows.  Sums in fp32, one rounding at the end, in
  * an order that depends on the arguments alone: equal calls give equal bits.  With accumulate, rows
  * that no id names are left as they are; without, they become zero.
- * V <= 2^31 - 1 (gradient: 2^31 - 2), n <= 2^31 - 1 (gradient).
+ * D <= 2^26, V <= 2^31 - 1 (gradient: 2^31 - 2), n <= 2^31 - 1 (gradient).
  * ------------------------------------------------------------------------------------- */
 int ddg_embedding(const void *ids, int ids_64, int64_t n, const void *table, int table_type, int64_t V, int D,
                   int64_t ld_table, float scale, void *out, int out_type, int64_t ld_out, void *stream);
@@ -594,10 +594,14 @@ int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, int state_bit
  *   dX = Q(dY) Q(W)                dY in groups along a row
  *   dW = Q'(dY)^T Q'(X)            groups of 128 along the batch;  db = column sums of dY in fp32
  * A block's scale is the smallest power of two that brings its largest magnitude to 448 or below;
- * a block whose largest magnitude is below 2^-100 counts as zeros.  Infinities and NaN give NaN.
+ * a block whose largest magnitude is below 2^-100 counts as zeros.  An infinity or a NaN gives NaN where
+ * it is multiplied; beside an infinity the finite elements of its block count as zeros.
+ * Products of bf16 results drop bits below about 2^-14 of a block's largest product, far below the
+ * result's rounding; all other results are sums of exact products in fp32.
+ * Reductions (in; out and rows for the gradients) shorter than 2^24, else DDG_E_UNSUPPORTED.
  * Packed operand [rows, cols]: ddg_fp8_operand_bytes(rows, cols) bytes, aligned to 256.
  * ddg_fp8_pack_weight: W -> packed [out, in] and, for the gradients, packed_t [in, out] (may be NULL).
- * dx and db may not be NULL / may be NULL.  A workspace is aligned to 256.
+ * db may be NULL.  A workspace is aligned to 256.
  * ------------------------------------------------------------------------------------- */
 size_t ddg_fp8_operand_bytes(int64_t rows, int64_t cols);
 int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t out, int64_t in, void *packed, void *packed_t,

@@ -299,3 +299,41 @@ def test_refusals(dev):
         with pytest.raises(DdgError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_large_tensors(dev, bits, max_norm):
+    """more than a million elements: four blocks per wave, the clip in a launch of its own"""
+    shapes = [(1100, 1001), (3,), (70001,), (1 << 20,)]
+    params, grads = tensors(shapes, BF16, 0.5, 20, dev), tensors(shapes, [BF16, F32, BF16, F32], 0.1, 21, dev)
+    opt = ops.AdamW(params, grads, weight_decay=[0.1, 0.0, 0.0, 0.1], max_norm=max_norm, state_bits=bits, masters=True, **H)
+    for _ in range(2):
+        before = snapshot(opt)
+        opt.step()
+        check_step(opt, before, grads)
+    if max_norm is None:
+        return
+    saved, old = {k: v.clone() for k, v in opt.state_dict().items()}, [p.clone() for p in params]
+    grads[2][70000] = float("inf")
+    assert not math.isfinite(float(opt.step()))
+    assert all(torch.equal(a, b) for a, b in zip(old, params))
+    assert all(torch.equal(v.view(torch.uint8), saved[k].view(torch.uint8)) for k, v in opt.state_dict().items())
+
+
+def test_nothing_but_empty_tensors(dev):
+    opt = ops.AdamW([torch.zeros(0, device=dev)], [torch.zeros(0, device=dev)], max_norm=1.0, state_bits=8)
+    assert float(opt.step()) == 0 and int(opt.step_count) == 1
+
+
+def test_steps_on_another_stream(dev):
+    """the handle made on one stream, used on another after a wait"""
+    make = lambda: ops.AdamW(tensors([(5000,)], F32, 0.5, 22, dev), tensors([(5000,)], F32, 0.1, 23, dev), max_norm=1.0, **H)
+    a, b = make(), make()
+    a.step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b.step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(a.params[0], b.params[0])

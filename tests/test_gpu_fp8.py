@@ -246,3 +246,62 @@ def test_refusals(dev):
         with pytest.raises(DdgError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("M,K,N", [(17, 8192, 1000), (40, 4200, 300), (300, 9000, 130), (128, 4096, 4096)])
+@pytest.mark.parametrize("ot", [F32, BF16, F16])
+def test_long_reductions_of_few_tiles(dev, M, K, N, ot):
+    """split reductions, whose parts are added in a second launch"""
+    x, W = data(M, K, 30, dev, BF16), data(N, K, 31, dev, BF16) * 0.02
+    bias = torch.randn(N, generator=torch.Generator(device=dev).manual_seed(32), device=dev)
+    w8 = ops.Fp8Weight(W)
+    y = ops.linear_fp8(x, w8, bias=bias, out_dtype=ot)
+    check_linear(x, W, bias, y)
+    assert torch.equal(y, ops.linear_fp8(x, w8, bias=bias, out_dtype=ot))
+    buf = torch.full((M, N + 5), 2.0, device=dev, dtype=ot)
+    ops.linear_fp8(x, w8, bias=bias, out=buf[:, 3:3 + N])
+    assert torch.equal(buf[:, 3:3 + N], y) and (buf[:, :3] == 2).all() and (buf[:, 3 + N:] == 2).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(20000, 176, 352), (9001, 100, 130), (33, 5000, 40), (33, 40, 5000), (3200, 3900, 520)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_grads_of_long_batches_and_wide_layers(dev, M, K, N, dt):
+    """split reductions over the batch (dW) and over the layer's output (dX); the last case has dX in 256 x 256 tiles"""
+    x, W, dy = data(M, K, 33, dev, dt, spread=0.3), data(N, K, 34, dev, dt) * 0.05, data(M, N, 35, dev, dt, spread=0.3)
+    w8 = ops.Fp8Weight(W)
+    dx, dw, db = ops.linear_fp8_grads(dy, x, w8, want_bias=True)
+    check_grads(x, W, dy, dx, dw, db)
+    again = ops.linear_fp8_grads(dy, x, w8, want_bias=True)
+    assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
+
+
+@pytest.mark.parametrize("M,K", [(1, 150000), (7, 40000), (16, 9001), (16, 9000)])
+def test_few_rows_of_long_reductions(dev, M, K):
+    """more blocks of x than fit a workgroup's LDS at a time"""
+    x, W = data(M, K, 36, dev, BF16), data(21, K, 37, dev, BF16) * 0.02
+    for ot in (F32, BF16):
+        check_linear(x, W, None, ops.linear_fp8(x, ops.Fp8Weight(W), out_dtype=ot))
+
+
+def test_reduction_with_offsets_past_31_bits(dev):
+    """rows of 9 million codes: a tile's last row begins beyond 2^31 bytes of its first"""
+    M, K, N = 260, 9000000, 3
+    x = torch.zeros(M, K, dtype=BF16, device=dev)
+    W = torch.zeros(N, K, dtype=BF16, device=dev)
+    at = torch.tensor([0, 127, 128, 4500000, K - 1], device=dev)
+    rows = torch.tensor([0, 238, 239, 255, 256, 259], device=dev)
+    x[rows[:, None], at] = data(6, 5, 38, dev, BF16)
+    W[:, at] = data(N, 5, 39, dev, BF16)
+    y = ops.linear_fp8(x, ops.Fp8Weight(W, grads=False), out_dtype=F32)
+    # (every element named is alone in its block or shares it with one other row's: scales as in the small problem of these columns)
+    ref = torch.zeros(M, N, dtype=torch.float64, device=dev)
+    for c in at.tolist():
+        lo, hi = c // 128 * 128, min(c // 128 * 128 + 128, K)
+        mine = [k for k in at.tolist() if lo <= k < hi]
+        if c != mine[0]:
+            continue
+        qx, qw = quantise(x[:, lo:hi], 1, 128)[0], quantise(W[:, lo:hi], 128, 128)[0]
+        ref += torch.mm(qx, qw.t().contiguous())
+    assert ((y.double() - ref).abs() <= 8 * 2.0 ** -24 * ref.abs() + 1e-6 * ref.abs().max()).all()
+    assert (y[1:238] == 0).all()
+

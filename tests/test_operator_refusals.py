@@ -84,6 +84,15 @@ def test_fp8_linear_refuses(kw, rc):
     assert fp8(**kw) == rc
 
 
+def test_fp8_reductions_that_are_too_long():
+    """refused in front of the first launch: these pointers are followed nowhere"""
+    assert fp8(rows=17, inn=1 << 24, ldx=1 << 24, wsb=1 << 62) == UNSUPPORTED
+    assert fp8(rows=1, inn=1 << 24, ldx=1 << 24, wsb=1 << 62) == UNSUPPORTED
+    g = lambda rows, out, inn: _lib.lib().ddg_fp8_linear_grads(P, 0, out, P, 0, inn, rows, P, out, inn, P, 0, inn, P, None, P, 1 << 62,
+                                                               None)
+    assert g(1 << 24, 32, 64) == UNSUPPORTED and g(50, 1 << 24, 64) == UNSUPPORTED
+
+
 def test_fp8_linear_no_rows():
     assert fp8(rows=0, x=None, y=None, ws=None, wsb=0) == OK
 
