@@ -242,11 +242,13 @@ __global__ __launch_bounds__(256) void k_f8_colsum(F8Colsum s) {
 // memory straight to LDS writes linearly, so the exchange is applied to the global address.  The scale words of four stages
 // lie behind the two stages.
 //
-// One barrier per stage, placed before the last column of tiles of stage k: by then every fragment of stage k has been read,
-// so its buffer takes stage k + 2, and stage k + 1 has landed, whose fragments are read between the matrix instructions of
-// that last column, each register right after its last use.  The copies of a stage are issued one by one between the matrix
-// instructions of two columns: issued in a row they hold up the instructions behind them, as a CU takes about 64 bytes of
-// them a cycle.
+// One barrier per stage, towards its end: by then every fragment of stage k has been read, so its buffer takes stage k + 2,
+// and stage k + 1 has landed, whose fragments are read between the matrix instructions behind the barrier.  Codes: the wave holds
+// its NT fragments of B and takes those of A one after the other, two steps of NT instructions behind the barrier (the other
+// way round, 18 reads of 16 bytes fall into a quarter of the stage, more than the LDS delivers: 8192 x 4096 x 8192 256 us
+// against 248).  Expanded: it holds A and takes B, one column behind the barrier, so that B is expanded bit by bit
+// (8192 x 4096 x 4096 235 us; the other way round 253).  The copies of a stage are issued one by one between the matrix
+// instructions: issued in a row they hold up the instructions behind them, as a CU takes about 64 bytes of them a cycle.
 template <int MT, int NT, int WM, int WN> struct F8Shape {
     static constexpr int WAVES = WM * WN, BM = MT * 16 * WM, BN = NT * 16 * WN, ROWS = BM + BN, LOADS = ROWS / 8 / WAVES,
                          LOADS_A = BM / 8 / WAVES, STAGE = ROWS * F8_BLOCK, STAGES = 2 * STAGE + 2 * ROWS * 4;
@@ -367,65 +369,118 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     };
 
     f32x4 acc[NT][MT] = {};
-    i32x8 fa[MT], fb;
-    uint32_t ea[MT], eb;
-    constexpr int HALF = S::LOADS / 2, EVERY = HALF < MT ? MT / HALF : 1;
-    static_assert(S::LOADS % 2 == 0 && HALF * EVERY <= MT, "half a stage's copies in a column of tiles");
+    constexpr int HALF = S::LOADS / 2;
+    static_assert(S::LOADS % 2 == 0, "half a stage's copies at a time");
 #pragma unroll
     for (int i = 0; i <= S::LOADS; ++i) copy(0, 0, i);
 #pragma unroll
     for (int i = 0; i < HALF; ++i) copy(nk > 1 ? 1 : 0, 1, i);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    // copy number `slot` of `slots` places, in the last steps of stage k (the first half of stage k + 2) and in the first ones
+    // (the second half of stage k + 1, and its scale words)
+    auto copy_last = [&](int k, int slot, int slots) {
+        const int every = slots / HALF;
+        if (slot % every == every - 1 && slot / every < HALF) copy(k + 2 < nk ? k + 2 : nk - 1, k & 1, slot / every);
+    };
+    auto copy_first = [&](int k, int slot, int slots) {
+        const int every = slots / HALF, to = k + 1 < nk ? k + 1 : nk - 1;
+        if (slot % every == every - 1 && slot / every < HALF) copy(to, (k + 1) & 1, HALF + slot / every);
+        if (slot == slots - 1) copy(to, (k + 1) & 1, S::LOADS);
+    };
+    // The matrix instructions' first operand: rows of the result = n, so that a lane gets four consecutive n.  The order of the
+    // statements is the schedule: nothing moves across the sched_barriers.  (Behind the last stage: read and not used.)
+    if constexpr (EXPAND) {
+        i32x8 fa[MT], fb;
+        uint32_t ea[MT], eb;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        fa[i] = frag(lo_a, hi_a, 0, i);
-        ea[i] = scale(sc_a, 0, i);
-    }
-    fb = frag(lo_b, hi_b, 0, 0);
-    eb = scale(sc_b, 0, 0);
-    for (int k = 0; k < nk; ++k) {
-        bf16x8 xa[EXPAND ? MT : 1][4];
-        if constexpr (EXPAND)
+        for (int i = 0; i < MT; ++i) {
+            fa[i] = frag(lo_a, hi_a, 0, i);
+            ea[i] = scale(sc_a, 0, i);
+        }
+        fb = frag(lo_b, hi_b, 0, 0);
+        eb = scale(sc_b, 0, 0);
+        for (int k = 0; k < nk; ++k) {
+            bf16x8 xa[MT][4];
 #pragma unroll
             for (int i = 0; i < MT; ++i) f8_expand(fa[i], ea[i], xa[i]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            bf16x8 xb[4];
-            if constexpr (EXPAND) f8_expand(fb, eb, xb);
-            const i32x8 cb = fb;
-            const uint32_t ce = eb;
-            if (j + 1 < NT) {
-                fb = frag(lo_b, hi_b, k, j + 1);
-                eb = scale(sc_b, k, j + 1);
-            } else {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                fb = frag(lo_b, hi_b, k + 1, 0);        // (behind the last stage: read and not used)
-                eb = scale(sc_b, k + 1, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            // first operand of the instructions: rows of the result = n, so that a lane gets four consecutive n
+            for (int j = 0; j < NT; ++j) {
+                bf16x8 xb[4];
+                f8_expand(fb, eb, xb);
+                if (j + 1 == NT) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                fb = frag(lo_b, hi_b, j + 1 < NT ? k : k + 1, j + 1 < NT ? j + 1 : 0);
+                eb = scale(sc_b, j + 1 < NT ? k : k + 1, j + 1 < NT ? j + 1 : 0);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if constexpr (EXPAND) {
+                for (int i = 0; i < MT; ++i) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[u], xa[i][u], acc[j][i], 0, 0, 0);
-                } else {
-                    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(cb, fa[i], acc[j][i], 0, 0, 0, (int)ce, 0,
+                    if (j + 1 == NT) {
+                        fa[i] = frag(lo_a, hi_a, k + 1, i);
+                        ea[i] = scale(sc_a, k + 1, i);
+                        copy_last(k, i, MT);
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else if (j == 0) {
+                        copy_first(k, i, MT);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    } else {
+        constexpr int WALL = MT - 2;                    // the barrier stands before this step
+        i32x8 fb0[NT], fb1[NT], next_a;                 // fragments that a stage begins with, and their scales
+        uint32_t e0[NT], e1[NT], next_ea;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            fb0[j] = frag(lo_b, hi_b, 0, j);
+            e0[j] = scale(sc_b, 0, j);
+        }
+        next_a = frag(lo_a, hi_a, 0, 0);
+        next_ea = scale(sc_a, 0, 0);
+        auto stage = [&](int k, const i32x8(&b)[NT], const uint32_t(&e)[NT], i32x8(&bn)[NT], uint32_t(&en)[NT]) {
+            i32x8 a[MT];
+            uint32_t ea[MT];
+            a[0] = next_a;
+            ea[0] = next_ea;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if (i == WALL) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+                for (int r = 0; r < MT; ++r)            // one step ahead; the last two of them before the barrier
+                    if (r == i + 1 ? r < WALL : r == WALL ? i == WALL - 2 : r == WALL + 1 && i == WALL - 1) {
+                        a[r] = frag(lo_a, hi_a, k, r);
+                        ea[r] = scale(sc_a, k, r);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i], acc[j][i], 0, 0, 0, (int)e[j], 0,
                                                                                 (int)ea[i]);
-                }
-                if (j + 1 == NT) {
-                    fa[i] = frag(lo_a, hi_a, k + 1, i);
-                    ea[i] = scale(sc_a, k + 1, i);
-                    if (i % EVERY == EVERY - 1 && i / EVERY < HALF) copy(k + 2 < nk ? k + 2 : nk - 1, k & 1, i / EVERY);
-                    __builtin_amdgcn_sched_barrier(0);  // not earlier: the register is in use until here
-                }
-                if (j == 0) {
-                    if (i % EVERY == EVERY - 1 && i / EVERY < HALF) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, HALF + i / EVERY);
-                    if (i == MT - 1) copy(k + 1 < nk ? k + 1 : nk - 1, (k + 1) & 1, S::LOADS);
+                    const int slot = (i < WALL ? i : i - WALL) * NT + j;
+                    if (i >= WALL) {
+                        if (slot % 2 == 0) {
+                            bn[slot / 2] = frag(lo_b, hi_b, k + 1, slot / 2);
+                            en[slot / 2] = scale(sc_b, k + 1, slot / 2);
+                        }
+                        if (slot == 2 * NT - 1) {
+                            next_a = frag(lo_a, hi_a, k + 1, 0);
+                            next_ea = scale(sc_a, k + 1, 0);
+                        }
+                        copy_last(k, slot, 2 * NT);
+                    } else if (i < 2) {
+                        copy_first(k, slot, 2 * NT);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+        };
+        for (int k = 0;; k += 2) {
+            stage(k, fb0, e0, fb1, e1);
+            if (k + 1 >= nk) break;
+            stage(k + 1, fb1, e1, fb0, e0);
+            if (k + 2 >= nk) break;
         }
     }
     // The copies behind the last stage end here, and the stages' memory becomes the waves' own: a wave turns its tile around in
