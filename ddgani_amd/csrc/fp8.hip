@@ -100,7 +100,7 @@ template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F
     const int64_t ld = p.ld, rows = p.rows, cols = p.cols;
     uint8_t *const q = p.q, *const s = p.s, *const qt = p.qt, *const st = p.st;
     float *const sums = p.sums;
-    __shared__ float red[16][F8_BLOCK];
+    __shared__ float red[2][4][F8_BLOCK];
     __shared__ uint8_t tr[F8_BLOCK][F8_BLOCK + 8];
     const int tc = threadIdx.x & 15, tr8 = (threadIdx.x >> 4) * 8;
     const int64_t tiles_c = (cols + F8_BLOCK - 1) / F8_BLOCK, rb = tile / tiles_c, cb = tile - rb * tiles_c;
@@ -108,42 +108,50 @@ template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F
     const int64_t cp = f8_pad(cols), rp = f8_pad(rows);
     const int nc = cols - c >= 8 ? 8 : cols > c ? (int)(cols - c) : 0;
     float v[8][8];
+    if (cols % 8 == 0) {                                // a thread's eight columns exist or not, together: no branch between loads
+        vec8<T> t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_n<8>(x + (r0 + tr8 + i) * ld + c, r0 + tr8 + i < rows ? nc : 0, v[i]);
+        for (int i = 0; i < 8; ++i) t[i] = load_whole(x + (r0 + tr8 + i < rows ? r0 + tr8 + i : rows - 1) * ld + (nc ? c : 0));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = nc && r0 + tr8 + i < rows ? (float)t[i][j] : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_n<8>(x + (r0 + tr8 + i) * ld + c, r0 + tr8 + i < rows ? nc : 0, v[i]);
+    }
 
+    // column maxima (and sums) of the tile: over the thread's eight rows, the four row groups of a wave, the four waves
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[i][j]));
+        a = fmaxf(a, __shfl_xor(a, 16));
+        a = fmaxf(a, __shfl_xor(a, 32));
+        if (lane < 16) red[0][wave][tc * 8 + j] = a;
+    }
     if (sums) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float a = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) a += v[i][j];
-            red[threadIdx.x >> 4][tc * 8 + j] = a;
+            a += __shfl_xor(a, 16);
+            a += __shfl_xor(a, 32);
+            if (lane < 16) red[1][wave][tc * 8 + j] = a;
         }
-        __syncthreads();
-        if (threadIdx.x < F8_BLOCK && c0 + threadIdx.x < cols) {
-            float a = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) a += red[i][threadIdx.x];
-            sums[rb * cols + c0 + threadIdx.x] = a;
-        }
-        __syncthreads();
-    }
-    // column maxima of the tile (their maximum in F8_TILE)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float a = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[i][j]));
-        red[threadIdx.x >> 4][tc * 8 + j] = a;
     }
     __syncthreads();
+    if (sums && threadIdx.x < F8_BLOCK && c0 + threadIdx.x < cols) {
+        const int t = threadIdx.x;
+        sums[rb * cols + c0 + t] = (red[1][0][t] + red[1][1][t]) + (red[1][2][t] + red[1][3][t]);
+    }
     float top[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        top[j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top[j] = fmaxf(top[j], red[i][tc * 8 + j]);
-    }
+    for (int j = 0; j < 8; ++j)
+        top[j] = fmaxf(fmaxf(red[0][0][tc * 8 + j], red[0][1][tc * 8 + j]), fmaxf(red[0][2][tc * 8 + j], red[0][3][tc * 8 + j]));
     int e[8];
     if (MODE == F8_TILE) {
         float a = 0.f;
@@ -199,10 +207,10 @@ template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F
     }
 }
 
-template <class T> __global__ __launch_bounds__(256) void k_f8_pack_weight(F8Pack w) { f8_pack_one<T, F8_TILE>(w, blockIdx.x); }
+template <class T> __global__ __launch_bounds__(256, 4) void k_f8_pack_weight(F8Pack w) { f8_pack_one<T, F8_TILE>(w, blockIdx.x); }
 
 // the operands of both gradients in one launch: tiles of dy, then tiles of x (either may be none)
-template <class T> __global__ __launch_bounds__(256) void k_f8_pack_grads(F8Pack dy, uint32_t tiles_dy, F8Pack x) {
+template <class T> __global__ __launch_bounds__(256, 4) void k_f8_pack_grads(F8Pack dy, uint32_t tiles_dy, F8Pack x) {
     if (blockIdx.x < tiles_dy) f8_pack_one<T, F8_ROWS_COLS>(dy, blockIdx.x);
     else f8_pack_one<T, F8_COLS>(x, blockIdx.x - tiles_dy);
 }
