@@ -538,14 +538,15 @@ __global__ __launch_bounds__(64 * WM * WN, MT * NT <= 8 ? 3 : 2) void k_f8_gemm(
     f8_gemm_tile<MT, NT, WM, WN, EXPAND, TO>(g, blockIdx.x);
 }
 // dW (fp32) and dX of one layer, and db, in one launch: neither product has the tiles for whole rounds of the CUs.  db's
-// workgroups (`sums`, may be none) first, then dW's, the longer ones
+// workgroups (`sums`, may be none) first, then those of the product whose workgroups take longer
 template <int NT, bool EXPAND, class TO>
 __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void k_f8_gemm_grads(F8Gemm dw, F8Gemm dx, F8Colsum db, uint32_t sums) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const uint32_t first = dw.tiles_m * dw.tiles_n * dw.splits, id = blockIdx.x - sums;
+    const uint32_t nw = dw.tiles_m * dw.tiles_n * dw.splits, nx = dx.tiles_m * dx.tiles_n * dx.splits, id = blockIdx.x - sums;
+    const bool dx_first = dx.blocks * (EXPAND ? 2 : 1) > dw.blocks * 2;         // (codes: half the time for a block)
     if (blockIdx.x < sums) f8_colsum(db, blockIdx.x, (float *)lds);
-    else if (id < first) f8_gemm_tile<4, NT, 2, 2, true, float>(dw, id);
-    else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, id - first);
+    else if (dx_first ? id >= nx : id < nw) f8_gemm_tile<4, NT, 2, 2, true, float>(dw, dx_first ? id - nx : id);
+    else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, dx_first ? id : id - nw);
 }
 
 // C = bias + sum of the parts, in their order; four columns per thread
