@@ -191,7 +191,7 @@ struct AdwState {
 // A wave owns UNITS blocks of 256 elements, four consecutive elements per lane: every access is one contiguous piece per
 // wave, and a block's maximum is one reduction over the wave.  All loads come first.  Workgroups take the table from its end:
 // what the norm read last is still in the 256 MB cache, and in the wide variant everything but the gradients goes past it
-// (332 million elements 1 185 -> STREAMUS us).  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
+// (332 million elements 1 185 -> 1 112 us).  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
 // adds up the partial norms and forms the step's scalars itself, which is quicker than a launch of its own for them.
 // (One launch for norm and step, whose last workgroup to arrive goes on alone, is slower: an atomic that all XCDs share takes
 // 85 ns a workgroup.)
@@ -309,12 +309,14 @@ static int64_t adw_total(const ddg_adamw_tensor *t, int n_tensors, bool wide) {
 
 static int adw_check(const ddg_adamw_tensor *t, int n_tensors, int64_t state_len) {
     if (n_tensors < 0 || (n_tensors > 0 && !t) || state_len < 0) return DDG_E_ARG;
+    int64_t chunks = 0;
     for (int i = 0; i < n_tensors; ++i) {
         if (t[i].numel < 0 || t[i].offset < 0 || t[i].offset % ADW_BLOCK || t[i].numel > state_len ||
-            t[i].offset > state_len - t[i].numel || !ddg_type_ok(t[i].param_type) || !ddg_type_ok(t[i].grad_type))
+            t[i].offset > state_len - t[i].numel || !(t[i].weight_decay >= 0) || !ddg_type_ok(t[i].param_type) || !ddg_type_ok(t[i].grad_type))
             return DDG_E_ARG;
         if (t[i].numel > 0 && (!t[i].param || !t[i].grad)) return DDG_E_ARG;
-        if (ceil_div64(t[i].numel, adw_chunk(true)) > 0x7FFFFFFF / ADW_TABLE) return DDG_E_UNSUPPORTED;
+        chunks += ceil_div64(t[i].numel, adw_chunk(true));
+        if (chunks > ddg_max_grid(ADW_NT)) return DDG_E_UNSUPPORTED;
     }
     return DDG_OK;
 }

@@ -694,7 +694,7 @@ extern "C" size_t ddg_fp8_operand_bytes(int64_t rows, int64_t cols) {
 
 static int f8_pack_rows(const void *x, int type, int64_t ld, const F8Operand &o, hipStream_t s) {
     const int64_t groups = o.rows * (f8_pad(o.cols) / F8_BLOCK), grid = ceil_div64(groups, 16);
-    if (grid > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
+    if (grid > ddg_max_grid(256)) return DDG_E_UNSUPPORTED;
     return ddg_with_type(type, [&](auto t) {
         using T = decltype(t);
         k_f8_pack_rows<T><<<(unsigned)grid, 256, 0, s>>>((const T *)x, ld, o.rows, o.cols, o.q, o.s);
@@ -705,11 +705,12 @@ static int f8_pack_rows(const void *x, int type, int64_t ld, const F8Operand &o,
 static inline int64_t f8_tiles(int64_t rows, int64_t cols) { return ceil_div64(rows, F8_BLOCK) * ceil_div64(cols, F8_BLOCK); }
 
 #define F8_WORKGROUPS 512                               // two per CU
-// Reductions are addressed with 32-bit offsets within a workgroup's 256 rows; tiles are counted in 32 bits (with their splits:
-// only where there are fewer tiles than F8_WORKGROUPS).  Checked in front of an entry point's first launch.
+// Reductions are addressed with 32-bit offsets within a workgroup's 256 rows; both gradients' tiles and db's workgroups (at
+// most two for a tile of dW) fit one launch of 256 threads each.  Tiles of 128 x 64 and splits: only where there are fewer than
+// eight stages for each of F8_WORKGROUPS.  Checked in front of an entry point's first launch.
 #define F8_MAX_REDUCTION ((int64_t)1 << 24)
 static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
-    return f8_pad(cols) < F8_MAX_REDUCTION && ceil_div64(rows_a, 128) <= 0x0FFFFFFF / ceil_div64(rows_b, 64);
+    return f8_pad(cols) < F8_MAX_REDUCTION && ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128) < (1 << 22);
 }
 
 // Tiles are 256 x 256 (bf16 results only) once there are three quarters of a CU's worth of them; else 128 x 128, or 128 x 64 while
@@ -763,7 +764,6 @@ static inline int64_t f8_join_grid(const F8Join &j) { return j.splits > 1 ? ceil
 static int f8_join_parts(const F8Join &a, int type, const F8Join &b, hipStream_t s) {
     const int64_t ga = f8_join_grid(a), gb = f8_join_grid(b);
     if (ga + gb == 0) return DDG_OK;
-    if (ga + gb > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
     return ddg_with_type(type, [&](auto t) {
         k_f8_join<decltype(t)><<<(unsigned)(ga + gb), 256, 0, s>>>(a, (uint32_t)ga, b);
         DDG_CHECK_LAUNCH();
@@ -855,7 +855,7 @@ extern "C" int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t 
     if (packed_t) t = f8_operand(packed_t, in, out);
     const F8Operand o = f8_operand(packed, out, in);
     const int64_t tiles = f8_tiles(out, in);
-    if (tiles > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
+    if (tiles > ddg_max_grid(256)) return DDG_E_UNSUPPORTED;
     return ddg_with_type(type, [&](auto ty) {
         k_f8_pack_weight<decltype(ty)><<<(unsigned)tiles, 256, 0, (hipStream_t)stream>>>(
             F8Pack{W, ld, out, in, o.q, o.s, t.q, t.s, nullptr});
@@ -892,6 +892,7 @@ extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t r
                     constexpr int W = decltype(waves)::value;
                     const int piece = nk < most ? nk : most / W * W;        // (a wave's blocks stay its own from piece to piece)
                     const int bytes = (((int)rows * (piece * (F8_BLOCK + 1) + 16) + 15) & ~15) + W * 64 * 16;
+                    if (ceil_div64(out, 16) > ddg_max_grid(64 * W)) return (int)DDG_E_UNSUPPORTED;
                     const auto kernel = k_f8_skinny<TX, TO, W>;
                     const int rc = f8_lds(kernel, bytes);
                     if (rc) return rc;
@@ -960,7 +961,7 @@ extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, 
     const hipStream_t s = (hipStream_t)stream;
     const F8Operand gy = f8_operand(w.dy, rows, out), gyt = f8_operand(w.dyt, out, rows), xt = f8_operand(w.xt, in, rows);
     const int64_t tiles_dy = f8_tiles(rows, out), tiles_x = f8_tiles(rows, in), row_tiles = ceil_div64(rows, F8_BLOCK);
-    if (tiles_dy + tiles_x > 0x7FFFFFFF) return DDG_E_UNSUPPORTED;
+    if (tiles_dy + tiles_x > ddg_max_grid(256)) return DDG_E_UNSUPPORTED;
     // (one row tile: its column sums are the result)
     const F8Pack pd = {dy, ld_dy, rows, out, gy.q, gy.s, gyt.q, gyt.s, !db ? nullptr : row_tiles == 1 ? db : w.sums};
     const F8Pack px = {x, ld_x, rows, in, nullptr, nullptr, xt.q, xt.s, nullptr};

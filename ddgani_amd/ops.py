@@ -909,6 +909,8 @@ class AdamW:
         if len(decay) != len(self.params):
             raise _lib.DdgError("AdamW: one weight_decay, or one for each tensor")
         self.weight_decay = [float(w) for w in decay]
+        if not all(w >= 0 for w in self.weight_decay):
+            raise _lib.DdgError("AdamW: weight_decay >= 0")
         self.device = dev = self.params[0].device
         spans = sorted((_ptr(p), p.numel() * p.element_size()) for p in self.params if p.numel())
         if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
@@ -963,6 +965,8 @@ class AdamW:
         """one step; lr: for this and the following steps.  -> the gradients' norm before the clip, a float32 [1] device tensor
         that the next step overwrites (None without max_norm)"""
         if lr is not None:
+            if not lr >= 0:
+                raise _lib.DdgError("AdamW: lr >= 0")
             self.lr = lr
         clip = self.max_norm is not None
         _call(self.dev, lib().ddg_adamw_step, "ddg_adamw_step", *self._state, self.lr, *self.betas, self.eps,

@@ -542,7 +542,7 @@ int ddg_decode_table(const float *code, const uint8_t *m, const double *obs, con
  * independent of each other; ld_*: elements between rows.  Sums in fp32, one rounding at the end, in
  * an order that depends on the arguments alone: equal calls give equal bits.  With accumulate, rows
  * that no id names are left as they are; without, they become zero.
- * D <= 2^26, V <= 2^31 - 1 (gradient: 2^31 - 2), n <= 2^31 - 1 (gradient).
+ * D <= 2^26, V <= 2^31 - 1 (gradient: 2^31 - 2), n <= 2^31 - 1 (gradient).  out overlaps no input.
  * ------------------------------------------------------------------------------------- */
 int ddg_embedding(const void *ids, int ids_64, int64_t n, const void *table, int table_type, int64_t V, int D,
                   int64_t ld_table, float scale, void *out, int out_type, int64_t ld_out, void *stream);
@@ -568,7 +568,9 @@ int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const void *dy, i
  * control: DDG_ADAMW_CONTROL_BYTES of device memory, zeroed by the caller before the first step: int64 step count at byte 0,
  *   float norm of the last step at byte 8 (max_norm > 0).  The step number advances on the device,
  *   so a captured graph may be replayed.  If the norm is not finite nothing changes but `norm`.
- * tensors: HOST array, read before the call returns.  workspace: only for max_norm > 0.
+ *   (Squares are formed in fp32: so does a gradient above 1.8e19.)  Without a clip a gradient that is not finite reaches the state, in 8 bits that of its whole block.
+ * tensors: HOST array, read before the call returns; weight_decay >= 0.  Parameters and gradients do not overlap.
+ *   workspace: only for max_norm > 0.
  * ------------------------------------------------------------------------------------- */
 #define DDG_ADAMW_BLOCK 256
 #define DDG_ADAMW_CONTROL_BYTES 64
@@ -598,7 +600,8 @@ int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, int state_bit
  * it is multiplied; beside an infinity the finite elements of its block count as zeros.
  * Products of bf16 results drop bits below about 2^-14 of a block's largest product, far below the
  * result's rounding; all other results are sums of exact products in fp32.
- * Reductions (in; out and rows for the gradients) shorter than 2^24, else DDG_E_UNSUPPORTED.
+ * Reductions (in; out and rows for the gradients) shorter than 2^24, X of fewer than 2^35 elements and results of fewer than
+ * 2^22 tiles of 128 x 128, else DDG_E_UNSUPPORTED.  Results overlap no input.
  * Packed operand [rows, cols]: ddg_fp8_operand_bytes(rows, cols) bytes, aligned to 256.
  * ddg_fp8_pack_weight: W -> packed [out, in] and, for the gradients, packed_t [in, out] (may be NULL).
  * db may be NULL.  A workspace is aligned to 256.

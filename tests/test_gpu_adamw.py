@@ -337,3 +337,15 @@ def test_steps_on_another_stream(dev):
         b.step()
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(a.params[0], b.params[0])
+
+
+def test_refused_rate_leaves_the_handle(dev):
+    opt = ops.AdamW(tensors([(50,)], F32, 0.5, 24, dev), tensors([(50,)], F32, 0.1, 25, dev), **H)
+    for lr in (-1.0, float("nan")):
+        with pytest.raises(DdgError):
+            opt.step(lr=lr)
+    assert opt.lr == H["lr"] and int(opt.step_count) == 0
+    with pytest.raises(DdgError):
+        ops.AdamW(opt.params, opt.grads, weight_decay=-0.1, **H)
+    opt.step()
+    assert int(opt.step_count) == 1

@@ -239,3 +239,17 @@ def test_refusals(dev):
         with pytest.raises(DdgError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("n", [70, 5000])
+@pytest.mark.parametrize("pad", [None, 2])
+def test_grad_of_tokens_that_name_no_row(dev, n, pad):
+    """a batch of padding only: long runs of positions that belong to no row"""
+    g = gen(8)
+    ids = torch.full((n,), -1, dtype=torch.int64, device=dev)
+    ids[n // 2:] = 9 if pad is None else pad
+    dy = torch.randn(n, 19, generator=g, device=dev).to(BF16)
+    dy[0] = float("nan")
+    assert (ops.embedding_grad(ids, dy, 9, padding_idx=pad) == 0).all()
+    old = torch.randn(9, 19, generator=g, device=dev)
+    assert torch.equal(ops.embedding_grad(ids, dy, 9, padding_idx=pad, out=old.clone(), accumulate=True), old)

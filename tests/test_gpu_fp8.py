@@ -305,3 +305,32 @@ def test_reduction_with_offsets_past_31_bits(dev):
     assert ((y.double() - ref).abs() <= 8 * 2.0 ** -24 * ref.abs() + 1e-6 * ref.abs().max()).all()
     assert (y[1:238] == 0).all()
 
+
+@pytest.mark.parametrize("N", [3900, 3905])
+def test_wide_tiles_strided_with_bias(dev, N):
+    """256 x 256 tiles that end inside the matrix, operands and result at odd offsets"""
+    M, K = 3201, 333
+    wide, Ww = data(M, K + 9, 40, dev, BF16), data(N, K + 5, 41, dev, BF16) * 0.1
+    x, W = wide[:, 3:3 + K], Ww[:, 1:1 + K]
+    bias = torch.randn(N + 1, generator=torch.Generator(device=dev).manual_seed(42), device=dev)[1:]
+    buf = torch.full((M, N + 11), 5.0, device=dev, dtype=BF16)
+    ops.linear_fp8(x, ops.Fp8Weight(W), bias=bias, out=buf[:, 3:3 + N])
+    check_linear(x, W, bias, buf[:, 3:3 + N])
+    assert (buf[:, :3] == 5).all() and (buf[:, 3 + N:] == 5).all()
+
+
+def test_layers_on_two_streams(dev):
+    """two calls at once, each with its own workspace"""
+    x, W = data(900, 700, 43, dev, BF16), data(500, 700, 44, dev, BF16) * 0.1
+    w8, want = ops.Fp8Weight(W), []
+    for k in (1, 2):
+        want.append(ops.linear_fp8(x * k, w8, out_dtype=F32).clone())
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(ops.linear_fp8(x * (k + 1), w8, out_dtype=F32))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k]) for k in (0, 1) for y in got[k])

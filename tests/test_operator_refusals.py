@@ -116,6 +116,29 @@ def test_fp8_grads_refuse(kw, rc):
     assert _lib.lib().ddg_fp8_linear_grads(*a.values()) == rc
 
 
+def test_more_workgroups_than_a_launch_takes():
+    """refused in front of the first launch as well"""
+    assert embed(n=1 << 33, D=2048, ld=2048, ldo=2048) == UNSUPPORTED
+    assert grad(V=(1 << 31) - 2, D=1 << 20, ldd=1 << 20, ldo=1 << 20, wsb=1 << 62) == UNSUPPORTED
+    assert grad(n=(1 << 31) - 1, D=2048, ldd=2048, ldo=2048, wsb=1 << 62) == UNSUPPORTED
+    big = 1 << 40
+    assert adamw(t=[dict(n=big)], length=big, wsb=1 << 40) == UNSUPPORTED
+    assert adamw(t=[dict(n=1 << 32, off=i << 32) for i in range(20)], length=20 << 32, wsb=1 << 40) == UNSUPPORTED
+    assert fp8(rows=1 << 29, inn=128, ldx=128, wsb=1 << 62) == UNSUPPORTED               # tiles of the result
+    assert fp8(rows=1 << 28, inn=128, ldx=128, wsb=1 << 62) == UNSUPPORTED               # groups of x
+    assert fp8(rows=1, out=1 << 28, ldy=1 << 28, inn=2048, ldx=2048) == UNSUPPORTED
+    g = lambda rows, out, inn: _lib.lib().ddg_fp8_linear_grads(P, 0, out, P, 0, inn, rows, P, out, inn, P, 0, inn, P, None, P, 1 << 62,
+                                                               None)
+    assert g(1 << 23, (1 << 24) - 256, (1 << 24) - 256) == UNSUPPORTED
+    pack = lambda out, inn: _lib.lib().ddg_fp8_pack_weight(P, 1, inn, out, inn, P, None, None)
+    assert pack(1 << 29, 1 << 20) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("decay", [-0.1, float("nan")])
+def test_adamw_refuses_decay(decay):
+    assert adamw(t=[dict(wd=decay)]) == ARG
+
+
 def test_workspace_sizes_of_bad_shapes():
     L = _lib.lib()
     assert L.ddg_embedding_grad_workspace_bytes(-1, 4) == 0 and L.ddg_embedding_grad_workspace_bytes(4, 0) == 0
