@@ -798,14 +798,19 @@ static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, vo
     return rc ? rc : f8_join_parts(f8_joined(a, b, sp, parts, bias, c, ldc), type, F8Join{nullptr, 0, 0, 1, nullptr, nullptr, 0}, s);
 }
 
-// the gradients' products: dx [rows, in] over out, dw [out, in] over rows
+// The gradients' products: dx [rows, in] over out, dw [out, in] over rows.  Two launches, dx in 256 x 256 tiles, where there are
+// enough of those, dw's tiles fill three quarters of their rounds of two per CU, and dx's reduction is not short; in one launch
+// dx's tiles fill the rounds.  Measured at 20 000 rows, apart and together: 8192 x 8192 3 200 and 3 470 us, 6000 x 6000 1 879 and
+// 1 977, 3000 x 3000 (0.56 of its rounds) 653 and 563, 2048 x 5000 (in x out) 663 and 632, 5000 x 2048 730 and 632; 8192 x 1000 567
+// and 570, but 131 and 120 at 4 001 rows.
 struct F8GradSplits {
     bool apart, narrow;                 // two launches (dx in 256 x 256 tiles); 128 x 64 tiles
     F8Split dx, dw;
 };
 static inline F8GradSplits f8_grad_splits(int64_t rows, int64_t out, int64_t in, bool bf16) {
     F8GradSplits g;
-    g.apart = bf16 && f8_wide(rows, in);
+    const int64_t tw = ceil_div64(out, 128) * ceil_div64(in, 128);
+    g.apart = bf16 && f8_wide(rows, in) && out > 1024 && tw * 4 >= ceil_div64(tw, F8_WORKGROUPS) * F8_WORKGROUPS * 3;
     g.narrow = f8_stages(rows, in, out, 128) + f8_stages(out, in, rows, 128) < 8 * F8_WORKGROUPS;
     const int bn = g.narrow ? 64 : 128;
     const int64_t all = f8_stages(rows, in, out, bn) + f8_stages(out, in, rows, bn);

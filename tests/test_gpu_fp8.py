@@ -263,10 +263,10 @@ def test_long_reductions_of_few_tiles(dev, M, K, N, ot):
     assert torch.equal(buf[:, 3:3 + N], y) and (buf[:, :3] == 2).all() and (buf[:, 3 + N:] == 2).all()
 
 
-@pytest.mark.parametrize("M,K,N", [(20000, 176, 352), (9001, 100, 130), (33, 5000, 40), (33, 40, 5000), (3200, 3900, 520)])
+@pytest.mark.parametrize("M,K,N", [(20000, 176, 352), (9001, 100, 130), (33, 5000, 40), (33, 40, 5000), (3200, 3900, 520), (3100, 5200, 1300)])
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_grads_of_long_batches_and_wide_layers(dev, M, K, N, dt):
-    """split reductions over the batch (dW) and over the layer's output (dX); the last case has dX in 256 x 256 tiles"""
+    """split reductions over the batch (dW) and over the layer's output (dX); the last case has a dX of bf16 in 256 x 256 tiles"""
     x, W, dy = data(M, K, 33, dev, dt, spread=0.3), data(N, K, 34, dev, dt) * 0.05, data(M, N, 35, dev, dt, spread=0.3)
     w8 = ops.Fp8Weight(W)
     dx, dw, db = ops.linear_fp8_grads(dy, x, w8, want_bias=True)
