@@ -17,8 +17,10 @@
 // one, so only bf16 results come from them; for the others the codes are expanded to bf16, which holds code x scale exactly,
 // and multiplied by v_mfma_f32_16x16x32_bf16 (8e-9 on the same data) at half the rate.
 //
-// Packed operand of `rows` rows and a reduction of `cols`: codes [rows][colsp] (colsp = cols rounded up to 128, zeros
-// behind cols), then from the next multiple of 256 bytes the scales as biased exponents (2^(e - 127)), four consecutive
+// Packed operand of `rows` rows and a reduction of `cols`: codes of colsp columns (cols rounded up to 128, zeros behind cols),
+// for the product's first operand row by row; for its second (weights, and X in dW) in pieces of 16 rows x 128 columns, [row /
+// 16][column / 128], as the matrix instruction takes them: lane r + 16 g holds codes 32 g to 32 g + 31 of row r, the first 16 of all
+// lanes come first.  A wave loads such a piece as 2 KB in a row.  (Rows up to the next multiple of 16 are zeros.)  Then from the next multiple of 256 bytes the scales as biased exponents (2^(e - 127)), four consecutive
 // blocks in one word: word [block / 4][row], byte block % 4.  The 16 rows of a matrix tile are 16 consecutive words.  1 KB
 // behind the scales belongs to the operand too: a workgroup reads whole 256-row pieces of them.
 #include <type_traits>
@@ -32,7 +34,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 static __host__ __device__ __forceinline__ int64_t f8_pad(int64_t cols) { return (cols + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK; }
 static __host__ __device__ __forceinline__ size_t f8_codes_bytes(int64_t rows, int64_t cols) {
-    return ((size_t)rows * f8_pad(cols) + 255) & ~(size_t)255;
+    return ((size_t)(rows + 15) / 16 * 16 * f8_pad(cols) + 255) & ~(size_t)255;
 }
 static inline size_t f8_scale_bytes(int64_t rows, int64_t cols) {
     return (((size_t)rows * ((f8_pad(cols) / F8_BLOCK + 3) / 4) * 4) + 1024 + 255) & ~(size_t)255;
@@ -87,6 +89,7 @@ __global__ __launch_bounds__(256) void k_f8_pack_rows(const T *__restrict__ x, i
 
 // 128 x 128 tiles in registers, 8 x 8 elements per thread.  MODE F8_COLS: groups along the columns, packed transposed (qt, st);
 // F8_ROWS_COLS: those and groups along the rows (q, s); F8_TILE: one scale for the tile, packed both ways (qt may be NULL).
+// F8_ROWS_COLS packs a first operand (of either product), the others second operands.
 // sums (may be NULL): fp32 column sums of the tile, [row tile][cols].
 enum { F8_COLS, F8_ROWS_COLS, F8_TILE };
 struct F8Pack {
@@ -164,6 +167,19 @@ template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = f8_exponent(top[j]);
     }
+    // the codes in tr as a second operand: rows from row0 on of n, block `block` of `blocks`; 2 KB at a time
+    auto put_pieces = [&](uint8_t *to, int64_t row0, int64_t n, int64_t block, int64_t blocks) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tile = i * 2 + (threadIdx.x >> 7), part = threadIdx.x & 127;
+            if (row0 + tile * 16 < n) {
+                uint4 w;
+                __builtin_memcpy(&w, &tr[tile * 16 + (part & 15)][((part >> 4) & 3) * 32 + (part >> 6) * 16], 16);
+                *(uint4 *)(to + ((row0 / 16 + tile) * blocks + block) * (16 * F8_BLOCK) + part * 16) = w;
+            }
+        }
+    };
     if (MODE == F8_TILE || MODE == F8_ROWS_COLS) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -176,15 +192,18 @@ template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F
                 er = f8_exponent(row16_max(a));
             }
             const float inv = f8_inverse(er);
-            if (r < rows) {
-                uint2 w;
-                w.x = f8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-                w.y = f8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-                *(uint2 *)(q + r * cp + c) = w;
-                if (tc == 0) f8_put_scale(s, rows, r, cb, er);
-            }
+            uint2 w;
+            w.x = f8_pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+            w.y = f8_pack4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+            if (MODE == F8_TILE) *(uint2 *)&tr[tr8 + i][tc * 8] = w;
+            else if (r < rows) *(uint2 *)(q + r * cp + c) = w;
+            if (tc == 0 && r < rows) f8_put_scale(s, rows, r, cb, er);
         }
-        if (MODE == F8_TILE && !qt) return;
+        if (MODE == F8_TILE) {
+            put_pieces(q, r0, rows, cb, cp / F8_BLOCK);
+            if (!qt) return;
+            __syncthreads();
+        }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -194,6 +213,10 @@ template <class T, int MODE> __device__ __forceinline__ void f8_pack_one(const F
         w.y = f8_pack4(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv);
         *(uint2 *)&tr[tc * 8 + j][tr8] = w;
         if (tr8 == 0 && c + j < cols) f8_put_scale(st, cols, c + j, rb, e[j]);
+    }
+    if (MODE != F8_ROWS_COLS) {
+        put_pieces(qt, c0, cols, rb, rp / F8_BLOCK);
+        return;
     }
     __syncthreads();
 #pragma unroll
@@ -243,7 +266,8 @@ __global__ __launch_bounds__(256) void k_f8_colsum(F8Colsum s) {
 // ---------------------------------------------------------------------------------------------
 // A workgroup owns BM x BN of the result, a wave MT x NT tiles of 16 x 16; one block of the reduction is a stage.
 //
-// LDS image of a stage: rows of 128 bytes, whose eight 16-byte pieces are exchanged by f8_swap(row).  A 16-byte read is served
+// LDS image of a stage: B's pieces as they are packed, read by consecutive lanes at consecutive addresses.  A: rows of 128
+// bytes, whose eight 16-byte pieces are exchanged by f8_swap(row).  A 16-byte read is served
 // in groups of 16 lanes, 0-3 + 12-15 + 20-27 and so on; with a fragment's lanes (row lane % 16, pieces lane / 16 * 2 and + 1) such a
 // group asks for one piece of eight rows and for another one of the other eight, and f8_swap puts all 16 into different
 // banks.  (row / 2 % 8 alone, right for 16 consecutive lanes, had every read take twice its time.)  The copy from global
@@ -316,7 +340,7 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     const uint32_t tiles_m = g.tiles_m, tiles_n = g.tiles_n, split = id / (tiles_m * tiles_n);
     id -= split * tiles_m * tiles_n;
     const int64_t M = g.M, N = g.N, kp = g.kp, ldc = g.ldc, k0 = (int64_t)split * g.blocks;
-    const uint8_t *const A = g.A + k0 * F8_BLOCK, *const B = g.B + k0 * F8_BLOCK;
+    const uint8_t *const A = g.A + k0 * F8_BLOCK, *const B = g.B + k0 * (16 * F8_BLOCK);
     const uint32_t *const As = g.As + k0 / 4 * M, *const Bs = g.Bs + k0 / 4 * N;
     const float *const bias = g.bias;
     TO *const C = (TO *)g.C + split * M * N;
@@ -335,13 +359,13 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     const int nk = (int)(kp / F8_BLOCK - k0 < g.blocks ? kp / F8_BLOCK - k0 : g.blocks);
 
     const uint8_t *const a0 = A + m0 * kp, *const b0 = B + n0 * kp;
-    const int64_t rows_a = M - m0, rows_b = N - n0;
-    uint32_t off[S::LOADS];                             // rows behind the end repeat the last one
+    const int64_t last_a = M - m0 - 1, last_b = (N - n0 - 1) / 16;      // last row of A, last 16 rows of B
+    uint32_t off[S::LOADS];                             // rows behind the end repeat the last ones
 #pragma unroll
     for (int i = 0; i < S::LOADS; ++i) {
-        const int in = (i * S::WAVES + wave) * 8 + (lane >> 3), row = i < S::LOADS_A ? in : in - S::BM;
-        const int64_t last = (i < S::LOADS_A ? rows_a : rows_b) - 1;
-        off[i] = (uint32_t)(row < last ? row : last) * (uint32_t)kp + (((lane & 7) ^ f8_swap(in)) * 16);
+        const int eight = i * S::WAVES + wave, row = eight * 8 + (lane >> 3), tile = (eight - S::BM / 8) / 2;
+        off[i] = i < S::LOADS_A ? (uint32_t)(row < last_a ? row : last_a) * (uint32_t)kp + (((lane & 7) ^ f8_swap(row)) * 16)
+                                : (uint32_t)(tile < last_b ? tile : last_b) * (uint32_t)kp * 16 + (eight & 1) * 1024 + lane * 16;
     }
     const int srow = (wave < S::ROWS / 64 ? wave : S::ROWS / 64 - 1) * 64;        // (further waves copy the last piece again)
     const bool scale_a = srow < S::BM;
@@ -351,7 +375,7 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     // over themselves).  No branches around here: the compiler would move matrix instructions across them
     auto copy = [&](int k, int buf, int i) {
         if (i < S::LOADS) {
-            const uint8_t *base = (i < S::LOADS_A ? a0 : b0) + (int64_t)k * F8_BLOCK;
+            const uint8_t *base = i < S::LOADS_A ? a0 + (int64_t)k * F8_BLOCK : b0 + (int64_t)k * (16 * F8_BLOCK);
             uint32_t o = off[i];
             asm("" : "+s"(base), "+v"(o));              // scalar base and 32-bit offset: one register per copy and lane
             f8_copy16(base, o, lds0 + buf * S::STAGE + (i * S::WAVES + wave) * 8 * F8_BLOCK);
@@ -365,7 +389,7 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
     // first tile of either operand; the other tiles lie at constant distances
     const int r16 = lane & 15, swap = f8_swap(r16), g2 = (lane >> 4) * 2;
     const uint8_t *const lo_a = lds + (wm + r16) * F8_BLOCK + (g2 ^ swap) * 16, *const hi_a = lds + (wm + r16) * F8_BLOCK + ((g2 + 1) ^ swap) * 16;
-    const uint8_t *const lo_b = lo_a + (S::BM + wn - wm) * F8_BLOCK, *const hi_b = hi_a + (S::BM + wn - wm) * F8_BLOCK;
+    const uint8_t *const lo_b = lds + (S::BM + wn) * F8_BLOCK + lane * 16, *const hi_b = lo_b + 1024;
     const uint8_t *const sc_a = lds + 2 * S::STAGE + (wm + r16) * 4, *const sc_b = sc_a + (S::BM + wn - wm) * 4;
     auto frag = [&](const uint8_t *lo, const uint8_t *hi, int k, int tile) {
         const i32x4 x = *(const i32x4 *)(lo + (k & 1) * S::STAGE + tile * (16 * F8_BLOCK));
@@ -594,7 +618,7 @@ __global__ __launch_bounds__(64 * W) void k_f8_skinny(const TX *__restrict__ X, 
     const int64_t n0 = (int64_t)blockIdx.x * 16, nr = n0 + m < N ? n0 + m : N - 1;
     const int nk = (int)(kp / F8_BLOCK), pitch = piece * F8_BLOCK + 16;
     uint8_t *const ex = lds + M * pitch;
-    const uint8_t *const brow = B + nr * kp + (lane >> 4) * 32;
+    const uint8_t *const brow = B + n0 * kp + lane * 16;
     f32x4 acc = {};
     i32x8 fb[U];
     uint32_t eb[U];
@@ -602,7 +626,8 @@ __global__ __launch_bounds__(64 * W) void k_f8_skinny(const TX *__restrict__ X, 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * W < nk ? k0 + u * W : nk - 1;
-            __builtin_memcpy(&fb[u], __builtin_assume_aligned(brow + (int64_t)k * F8_BLOCK, 32), 32);
+            const i32x4 x = *(const i32x4 *)(brow + (int64_t)k * (16 * F8_BLOCK)), y = *(const i32x4 *)(brow + (int64_t)k * (16 * F8_BLOCK) + 1024);
+            fb[u] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
             eb[u] = Bs[(int64_t)(k >> 2) * N + nr] >> ((k & 3) * 8);
         }
     };

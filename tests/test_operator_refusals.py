@@ -148,9 +148,9 @@ def test_workspace_sizes_of_bad_shapes():
 
 
 def test_operand_layout_size():
-    # codes: rows x (cols up to 128); scales: one word for four blocks and row, and 1 KB; each part up to 256 bytes
-    assert _lib.lib().ddg_fp8_operand_bytes(3, 130) == 768 + 1280
-    assert _lib.lib().ddg_fp8_operand_bytes(100, 513) == 100 * 640 + 2048      # 5 blocks: two words a row
+    # codes: (rows up to 16) x (cols up to 128); scales: one word for four blocks and row, and 1 KB; each part up to 256 bytes
+    assert _lib.lib().ddg_fp8_operand_bytes(3, 130) == 16 * 256 + 1280
+    assert _lib.lib().ddg_fp8_operand_bytes(100, 513) == 112 * 640 + 2048      # 5 blocks: two words a row
 
 
 def test_python_front_end_refuses_host_tensors():
