@@ -602,21 +602,22 @@ template <class TO> __global__ __launch_bounds__(256) void k_f8_join(F8Join a, u
     else f8_join<float>(b, (int64_t)(blockIdx.x - first) * 256 + threadIdx.x);
 }
 
-// At most 16 rows: bound by the bytes of B and by latency, so one launch does the layer.  A workgroup owns 16 rows of B; its W
-// waves share the reduction, and their first codes of B are on the way while the workgroup quantises X into LDS (in pieces
-// of the reduction that fit), each element once: quantised by the lanes that multiply it, 16 rows at a time whatever their
-// number, X took longer than B.  Every result type takes the expanded product here: the matrix unit is idle either way.
+// Few rows, 16 at most (f8_skinny): bound by the bytes of B and by latency, so one launch does the layer.  A workgroup owns 16
+// rows of B; its W waves share the reduction, and their first codes of B are on the way while the workgroup quantises X into LDS,
+// each element once: quantised by the lanes that multiply it, 16 rows at a time whatever their number, X took longer than B.
+// Every result type takes the expanded product here: the matrix unit is idle either way.  One row of 4096 x 4096 in bf16: 5.1 us,
+// 3.3 TB/s (6.7 us with B row by row, where neighbouring lanes read different rows); 28672 x 8192 38 us, 6.1 TB/s.
 #define F8_SKINNY 16
 #define F8_SKINNY_LDS (140 * 1024)
 template <class TX, class TO, int W>
 __global__ __launch_bounds__(64 * W) void k_f8_skinny(const TX *__restrict__ X, int64_t ldx, int M, int64_t K, const uint8_t *__restrict__ B,
                                                       const uint32_t *__restrict__ Bs, int64_t N, int64_t kp,
-                                                      const float *__restrict__ bias, TO *__restrict__ C, int64_t ldc, int piece) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];       // [M][pitch] codes, [M][piece] exponents, [W][64] sums
+                                                      const float *__restrict__ bias, TO *__restrict__ C, int64_t ldc) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];       // [M][pitch] codes, [M][nk] exponents, [W][64] sums
     constexpr int U = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15;
     const int64_t n0 = (int64_t)blockIdx.x * 16, nr = n0 + m < N ? n0 + m : N - 1;
-    const int nk = (int)(kp / F8_BLOCK), pitch = piece * F8_BLOCK + 16;
+    const int nk = (int)(kp / F8_BLOCK), pitch = nk * F8_BLOCK + 16, groups = M * nk;
     uint8_t *const ex = lds + M * pitch;
     const uint8_t *const brow = B + n0 * kp + lane * 16;
     f32x4 acc = {};
@@ -626,71 +627,71 @@ __global__ __launch_bounds__(64 * W) void k_f8_skinny(const TX *__restrict__ X, 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * W < nk ? k0 + u * W : nk - 1;
-            const i32x4 x = *(const i32x4 *)(brow + (int64_t)k * (16 * F8_BLOCK)), y = *(const i32x4 *)(brow + (int64_t)k * (16 * F8_BLOCK) + 1024);
-            fb[u] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            const uint8_t *const b = brow + (int64_t)k * (16 * F8_BLOCK);
+            fb[u] = __builtin_shufflevector(*(const i32x4 *)b, *(const i32x4 *)(b + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
             eb[u] = Bs[(int64_t)(k >> 2) * N + nr] >> ((k & 3) * 8);
         }
     };
-    for (int p0 = 0; p0 < nk; p0 += piece) {
-        const int here = nk - p0 < piece ? nk - p0 : piece;
-        load(p0 + wave);
-        if (p0) __syncthreads();                        // the last piece has been read
-        auto quantise = [&](auto in_flight) {           // groups of 128 of this lane's 16, that many loaded at a time
-            constexpr int Q = decltype(in_flight)::value;
-            for (int g0 = threadIdx.x >> 4; g0 < M * here; g0 += W * 4 * Q) {
-                vec8<TX> v[Q];
+    load(wave);
+    const float per_row = 1.f / (float)nk;
+    auto quantise = [&](auto in_flight) {               // groups of 128 of this lane's 16, that many loaded at a time
+        constexpr int Q = decltype(in_flight)::value;
+        for (int g0 = threadIdx.x >> 4; g0 < groups; g0 += W * 4 * Q) {
+            vec8<TX> v[Q];
+            int row[Q], k[Q];
 #pragma unroll
-                for (int u = 0; u < Q; ++u) {
-                    const int g = g0 + u * W * 4, row = g / here, k = g - row * here;
-                    const int64_t c = (int64_t)(p0 + k) * F8_BLOCK + m * 8;
-                    const TX *p = X + (row < M ? row : 0) * ldx;
-                    if (K >= 8) v[u] = load_whole(p + (c + 8 <= K ? c : 0));
-                    if (K % 8 && c < K && c + 8 > K) {
+            for (int u = 0; u < Q; ++u) {
+                const int g = g0 + u * W * 4 < groups ? g0 + u * W * 4 : groups - 1;
+                row[u] = (int)(((float)g + 0.5f) * per_row);            // g / nk: g < 2^11, half a unit is more than the rounding
+                k[u] = g - row[u] * nk;
+                const int64_t c = (int64_t)k[u] * F8_BLOCK + m * 8;
+                const TX *const p = X + row[u] * ldx;
+                if (K >= 8) v[u] = load_whole(p + (c + 8 <= K ? c : 0));
+                if (K % 8 && c < K && c + 8 > K) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[u][i] = c + i < K ? p[c + i] : (TX)0.f;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < Q; ++u) {
-                    const int g = g0 + u * W * 4, row = g / here, k = g - row * here;
-                    if (g >= M * here) break;           // (whole groups of 16 lanes leave)
-                    const bool live = (int64_t)(p0 + k) * F8_BLOCK + m * 8 < K;
-                    float f[8], a = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        f[i] = live ? (float)v[u][i] : 0.f;
-                        a = fmaxf(a, fabsf(f[i]));
-                    }
-                    const int e = f8_exponent(row16_max(a));
-                    const float inv = f8_inverse(e);
-                    uint2 w;
-                    w.x = f8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-                    w.y = f8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-                    *(uint2 *)(lds + row * pitch + k * F8_BLOCK + m * 8) = w;
-                    if (m == 0) ex[row * piece + k] = (uint8_t)e;
+                    for (int i = 0; i < 8; ++i) v[u][i] = c + i < K ? p[c + i] : (TX)0.f;
                 }
             }
-        };
-        if (M * here <= W * 4) quantise(std::integral_constant<int, 1>());
-        else quantise(std::integral_constant<int, 4>());
-        __syncthreads();
-        const uint8_t *const arow = lds + (m < M ? m : 0) * pitch + (lane >> 4) * 32, *const erow = ex + (m < M ? m : 0) * piece;
-        for (int k0 = wave; k0 < here; k0 += U * W) {
-            if (k0 != wave) load(p0 + k0);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = k0 + u * W;
-                if (k >= here) break;
-                const i32x4 x = *(const i32x4 *)(arow + k * F8_BLOCK), y = *(const i32x4 *)(arow + k * F8_BLOCK + 16);
-                bf16x8 xa[4], xb[4];
-                f8_expand(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), erow[k], xa);
-                f8_expand(fb[u], eb[u] & 0xFF, xb);
+            for (int u = 0; u < Q; ++u) {
+                if (g0 + u * W * 4 >= groups) break;    // (whole groups of 16 lanes leave)
+                const bool live = (int64_t)k[u] * F8_BLOCK + m * 8 < K;
+                float f[8], a = 0.f;
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
+                for (int i = 0; i < 8; ++i) {
+                    f[i] = live ? (float)v[u][i] : 0.f;
+                    a = fmaxf(a, fabsf(f[i]));
+                }
+                const int e = f8_exponent(row16_max(a));
+                const float inv = f8_inverse(e);
+                uint2 w;
+                w.x = f8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+                w.y = f8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+                *(uint2 *)(lds + row[u] * pitch + k[u] * F8_BLOCK + m * 8) = w;
+                if (m == 0) ex[row[u] * nk + k[u]] = (uint8_t)e;
             }
         }
+    };
+    if (groups <= W * 4) quantise(std::integral_constant<int, 1>());
+    else if (groups <= W * 8) quantise(std::integral_constant<int, 2>());
+    else quantise(std::integral_constant<int, 4>());
+    __syncthreads();
+    const uint8_t *const arow = lds + (m < M ? m : 0) * pitch + (lane >> 4) * 32, *const erow = ex + (m < M ? m : 0) * nk;
+    for (int k0 = wave; k0 < nk; k0 += U * W) {
+        if (k0 != wave) load(k0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * W;
+            if (k >= nk) break;
+            const i32x4 x = *(const i32x4 *)(arow + k * F8_BLOCK), y = *(const i32x4 *)(arow + k * F8_BLOCK + 16);
+            bf16x8 xa[4], xb[4];
+            f8_expand(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), erow[k], xa);
+            f8_expand(fb[u], eb[u] & 0xFF, xb);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[t], xa[t], acc, 0, 0, 0);
+        }
     }
-    f32x4 *const part = (f32x4 *)(lds + ((M * (pitch + piece) + 15) & ~15));
+    f32x4 *const part = (f32x4 *)(lds + ((M * (pitch + nk) + 15) & ~15));
     part[wave * 64 + lane] = acc;
     __syncthreads();
     if (wave) return;
@@ -894,10 +895,20 @@ extern "C" int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t 
     });
 }
 
+// k_f8_skinny: X fits the LDS, and its quantisation by every workgroup (13 elements a ns, and 3 us a workgroup besides; one
+// workgroup per CU at a time) takes less than the detour over packed X and tiles, 18 us and with another result than bf16
+// 22 us.  Rows from which the tiles were quicker (bf16, in x out): 2048 x 2048 and 4096 x 4096 none, 8192 x 8192 nine, 14336 x 4096 thirteen, 4096 x 14336 six, 4096 x
+// 32000 one; 16 rows through 8192 x 8192 32 us here and 24 us there, through 4096 x 4096 10 and 14.
+static inline bool f8_skinny(int64_t rows, int64_t out, int64_t in, bool bf16) {
+    const int64_t nk = f8_pad(in) / F8_BLOCK;
+    return rows <= F8_SKINNY && rows * (nk * (F8_BLOCK + 1) + 16) <= F8_SKINNY_LDS &&
+           (rows * in / 13 + 3000) * (out > 4096 ? out : 4096) <= (int64_t)(bf16 ? 18000 : 22000) * 4096;
+}
+
 extern "C" size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t out, int64_t in) {
     if (!f8_dims_ok(rows, in) || !f8_dims_ok(out, 0) || in < 1 || out < 1) return 0;
-    if (rows <= F8_SKINNY) return 0;
-    // (the result's type decides about 256 x 256 tiles, which are not split: room for either)
+    if (f8_skinny(rows, out, in, true)) return 0;
+    // (the result's type decides about more rows there, and about 256 x 256 tiles, which are not split: room for either)
     return ddg_fp8_operand_bytes(rows, in) + f8_parts_bytes(f8_split_one(rows, out, in, false), rows, out);
 }
 
@@ -912,23 +923,21 @@ extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t r
     if (!f8_product_ok(rows, out, in)) return DDG_E_UNSUPPORTED;
     const F8Operand w = f8_operand((void *)packed_w, out, in);
     const hipStream_t s = (hipStream_t)stream;
-    if (rows <= F8_SKINNY)
+    if (f8_skinny(rows, out, in, y_type == DDG_BF16))
         return ddg_with_type(x_type, [&](auto tx) {
             return ddg_with_type(y_type, [&](auto to) {
                 using TX = decltype(tx);
                 using TO = decltype(to);
-                const int nk = (int)(f8_pad(in) / F8_BLOCK), most = F8_SKINNY_LDS / (F8_BLOCK + 1) / (int)rows;
+                const int nk = (int)(f8_pad(in) / F8_BLOCK);
                 auto go = [&](auto waves) {
                     constexpr int W = decltype(waves)::value;
-                    const int piece = nk < most ? nk : most / W * W;        // (a wave's blocks stay its own from piece to piece)
-                    const int bytes = (((int)rows * (piece * (F8_BLOCK + 1) + 16) + 15) & ~15) + W * 64 * 16;
-                    if (ceil_div64(out, 16) > ddg_max_grid(64 * W)) return (int)DDG_E_UNSUPPORTED;
+                    const int bytes = (((int)rows * (nk * (F8_BLOCK + 1) + 16) + 15) & ~15) + W * 64 * 16;
                     const auto kernel = k_f8_skinny<TX, TO, W>;
                     const int rc = f8_lds(kernel, bytes);
                     if (rc) return rc;
                     kernel<<<(unsigned)ceil_div64(out, 16), 64 * W, bytes, s>>>((const TX *)x, ld_x, (int)rows, in, w.q,
                                                                                (const uint32_t *)w.s, out, f8_pad(in), bias, (TO *)y,
-                                                                               ld_y, piece);
+                                                                               ld_y);
                     DDG_CHECK_LAUNCH();
                     return (int)DDG_OK;
                 };

@@ -823,7 +823,7 @@ class Fp8Weight:
 
 def linear_fp8(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype] = None, out=None):
     """ddg_fp8_linear: x [rows, in] times the packed weight, + bias (float32 [out]) -> [rows, out] in out_dtype (default: x's).
-    x is quantised within the call, in groups of 128 along its rows; up to 16 rows take one launch."""
+    x is quantised within the call, in groups of 128 along its rows; few rows (up to 16) take one launch."""
     xp, ld = _matrix(x, "x")
     rows, inn = x.shape
     outd = weight.out_dim

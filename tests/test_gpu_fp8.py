@@ -275,9 +275,9 @@ def test_grads_of_long_batches_and_wide_layers(dev, M, K, N, dt):
     assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
 
 
-@pytest.mark.parametrize("M,K", [(1, 150000), (7, 40000), (16, 9001), (16, 9000)])
+@pytest.mark.parametrize("M,K", [(1, 150000), (7, 40000), (16, 9001), (16, 8704), (1, 140001), (3, 46000)])
 def test_few_rows_of_long_reductions(dev, M, K):
-    """more blocks of x than fit a workgroup's LDS at a time"""
+    """on either side of what fits a workgroup's LDS"""
     x, W = data(M, K, 36, dev, BF16), data(21, K, 37, dev, BF16) * 0.02
     for ot in (F32, BF16):
         check_linear(x, W, None, ops.linear_fp8(x, ops.Fp8Weight(W), out_dtype=ot))
@@ -334,3 +334,11 @@ def test_layers_on_two_streams(dev):
                 got[k].append(ops.linear_fp8(x * (k + 1), w8, out_dtype=F32))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[k]) for k in (0, 1) for y in got[k])
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 300, 40000), (5, 300, 20000), (5, 300, 30000), (16, 4096, 5000)])
+def test_few_rows_of_wide_layers(dev, M, K, N):
+    """on either side of the rule for the launch of few rows, with and without a workspace"""
+    x, W = data(M, K, 45, dev, BF16), data(N, K, 46, dev, BF16) * 0.02
+    for ot in (F32, BF16):
+        check_linear(x, W, None, ops.linear_fp8(x, ops.Fp8Weight(W), out_dtype=ot))
