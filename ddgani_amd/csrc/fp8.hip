@@ -739,15 +739,26 @@ static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
     return f8_pad(cols) < F8_MAX_REDUCTION && ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128) < (1 << 22);
 }
 
-// Tiles are 256 x 256 (bf16 results only) once there are three quarters of a CU's worth of them; else 128 x 128, or 128 x 64 while
-// all tiles together have fewer than eight stages for each of 512 workgroups: there the time is latency.  A tile whose reduction
+// Tiles are 256 x 256 (bf16 results only) once there are three quarters of a CU's worth of them and their rounds (one per CU)
+// cost less than those of 128 x 128 tiles (two per CU, two thirds of the time a round: 40 000 x 176 x 352 30.8 us with 256 x 256,
+// 25.3 with 128 x 128; 8192 x 4096 x 8192 is four rounds and eight); else 128 x 128, or 128 x 64 while
+// all tiles together have fewer than eight stages for each of 512 workgroups: there the time is latency.  Not where 128 x 128 tiles
+// come near one for each of those and cover no more columns (20 000 x 176 x 352 22.7 us with 128 x 64, 18.5 with 128 x 128; 40 000 x
+// 352 x 176, a third more columns, 33.5 and 36.2).  A tile whose reduction
 // takes twice its share of all stages and more is split into parts of about that share (a whole number of scale words, so
 // four stages at least), which are added afterwards, where that saves more (0.6 us a stage) than it costs (a launch, 3 us, and
 // the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 13.7 us, 128 x 4096 x 4096
 // 36 -> 24 us; 256 x 1000 x 8192 would go from 16 to 21 us and is left whole.
-static inline bool f8_wide(int64_t rows_a, int64_t rows_b) { return ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256) >= 192; }
+static inline bool f8_wide(int64_t rows_a, int64_t rows_b) {
+    const int64_t wide = ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256), small = ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128);
+    return wide >= 192 && ceil_div64(wide, 256) * 3 < ceil_div64(small, F8_WORKGROUPS) * 2;
+}
 static inline int64_t f8_stages(int64_t rows_a, int64_t rows_b, int64_t cols, int bn) {
     return ceil_div64(rows_a, 128) * ceil_div64(rows_b, bn) * (f8_pad(cols) / F8_BLOCK);
+}
+static inline bool f8_narrow(int64_t rows_a, int64_t rows_b, int64_t cols) {
+    const bool many = ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128) >= 400 && ceil_div64(rows_b, 128) * 2 == ceil_div64(rows_b, 64);
+    return !many && f8_stages(rows_a, rows_b, cols, 128) < 8 * F8_WORKGROUPS;
 }
 struct F8Split {
     int64_t splits, blocks;
@@ -761,7 +772,7 @@ static inline F8Split f8_split(int64_t m, int64_t n, int64_t cols, int64_t all_s
 // the split of a product on its own
 static inline F8Split f8_split_one(int64_t rows_a, int64_t rows_b, int64_t cols, bool bf16) {
     if (bf16 && f8_wide(rows_a, rows_b)) return {1, ceil_div64(f8_pad(cols) / F8_BLOCK, 4) * 4};
-    const bool narrow = f8_stages(rows_a, rows_b, cols, 128) < 8 * F8_WORKGROUPS;
+    const bool narrow = f8_narrow(rows_a, rows_b, cols);
     return f8_split(rows_a, rows_b, cols, f8_stages(rows_a, rows_b, cols, narrow ? 64 : 128));
 }
 static inline size_t f8_parts_bytes(const F8Split &sp, int64_t m, int64_t n) {
@@ -799,7 +810,7 @@ static int f8_join_parts(const F8Join &a, int type, const F8Join &b, hipStream_t
 
 static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int type, int64_t ldc, float *parts, hipStream_t s) {
     const F8Split sp = f8_split_one(a.rows, b.rows, a.cols, type == DDG_BF16);
-    const bool narrow = f8_stages(a.rows, b.rows, a.cols, 128) < 8 * F8_WORKGROUPS;
+    const bool narrow = f8_narrow(a.rows, b.rows, a.cols);
     auto go = [&](auto mt, auto nt, auto wm, auto wn, auto expand, auto to) {
         using TO = decltype(to);
         constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
