@@ -201,19 +201,14 @@ __device__ __forceinline__ uint64_t match_digit(uint32_t d, bool live, int digit
 
 // One wave places the pairs of [lo, hi) in their order; next[digit] is the wave's next free place.  A volatile pointer: the
 // wave's LDS accesses are executed in program order, so the count of one group of 64 is seen by the next.  Four groups are
-// loaded at a time.
-template <class GetK, class GetP, class Put>
+// loaded at a time, by get(first, k, p), the first four by the caller, the others while the four before them are placed.
+template <class Get, class Put>
 __device__ __forceinline__ void place_segment(int64_t lo, int64_t hi, int shift, int digit_bits, volatile uint32_t *next,
-                                              const GetK &getk, const GetP &getp, const Put &put) {
+                                              uint32_t (&k)[4], uint32_t (&p)[4], const Get &get, const Put &put) {
     const int lane = threadIdx.x & 63;
     for (int64_t g0 = lo; g0 < hi; g0 += 256) {
-        uint32_t k[4], p[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int64_t i = g0 + u * 64 + lane;
-            k[u] = i < hi ? getk(i) : 0;
-            p[u] = i < hi ? getp(i) : 0;
-        }
+        uint32_t k1[4] = {}, p1[4] = {};
+        if (g0 + 256 < hi) get(g0 + 256, k1, p1);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             if (g0 + u * 64 >= hi) break;
@@ -227,6 +222,11 @@ __device__ __forceinline__ void place_segment(int64_t lo, int64_t hi, int shift,
                 if (rank == 0) next[d] = at + __popcll(m);
             }
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            k[u] = k1[u];
+            p[u] = p1[u];
+        }
     }
 }
 
@@ -237,19 +237,19 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_scatter(SortSrc<ID> src, int64
     __shared__ uint32_t next[SORT_WAVES][SORT_BINS];
     __shared__ uint32_t wsum[SORT_WAVES];
     const int t = threadIdx.x, w = t >> 6, bins = 1 << digit_bits;
-    for (int i = 0; i < SORT_WAVES; ++i) next[i][t] = 0;
-    __syncthreads();
     const int64_t lo = blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n, seg = tile / SORT_WAVES;
     const int64_t slo = lo + w * seg < hi ? lo + w * seg : hi, shi = slo + seg < hi ? slo + seg : hi;
-    for (int64_t i0 = slo + (t & 63); i0 < shi; i0 += 256) {
-        uint32_t k[4];
+    auto get = [&](int64_t first, uint32_t (&k)[4], uint32_t (&p)[4]) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = i0 + u * 64 < shi ? src.k(i0 + u * 64) : 0;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i0 + u * 64 < shi) atomicAdd(&next[w][(k[u] >> shift) & (bins - 1)], 1u);
-    }
-    uint32_t before = 0, total = 0;
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = first + u * 64 + (t & 63);
+            k[u] = i < shi ? src.k(i) : 0;
+            p[u] = i < shi ? src.p(i) : 0;
+        }
+    };
+    // the segment's first pairs (all of them, up to 262 144 tokens) and the counts of the tiles are on the way together
+    uint32_t k[4], p[4], before = 0, total = 0;
+    get(slo, k, p);
     if (t < bins)
         for (int b = 0; b < tiles; b += 32) {           // (32 loads in flight: a loop of single ones took 30 us)
             uint32_t h[32];
@@ -261,7 +261,18 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_scatter(SortSrc<ID> src, int64
                 if (b + u < (int)blockIdx.x) before += h[u];
             }
         }
+    for (int i = 0; i < SORT_WAVES; ++i) next[i][t] = 0;
     __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (slo + u * 64 + (t & 63) < shi) atomicAdd(&next[w][(k[u] >> shift) & (bins - 1)], 1u);
+    for (int64_t i0 = slo + 256; i0 < shi; i0 += 256) {
+        uint32_t more[4], unused[4];
+        get(i0, more, unused);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * 64 + (t & 63) < shi) atomicAdd(&next[w][(more[u] >> shift) & (bins - 1)], 1u);
+    }
     uint32_t at = block_exclusive(total, wsum) + before;
     for (int i = 0; i < SORT_WAVES; ++i) {
         const uint32_t c = next[i][t];
@@ -269,11 +280,10 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_scatter(SortSrc<ID> src, int64
         at += c;
     }
     __syncthreads();
-    place_segment(slo, shi, shift, digit_bits, next[w], [&](int64_t i) { return src.k(i); }, [&](int64_t i) { return src.p(i); },
-                  [&](uint32_t d, uint32_t k, uint32_t p) {
-                      okey[d] = k;
-                      opos[d] = p;
-                  });
+    place_segment(slo, shi, shift, digit_bits, next[w], k, p, get, [&](uint32_t d, uint32_t key, uint32_t pos) {
+        okey[d] = key;
+        opos[d] = pos;
+    });
 }
 
 // n <= SORT_SMALL: every pass in LDS, one workgroup, one launch
@@ -306,11 +316,20 @@ __global__ __launch_bounds__(SORT_NT) void k_embg_sort_small(const ID *__restric
             at += c;
         }
         __syncthreads();
-        place_segment(slo, shi, shift, digit_bits, next[w], [&](int64_t i) { return key[a][i]; },
-                      [&](int64_t i) { return (uint32_t)pos[a][i]; }, [&](uint32_t d, uint32_t k, uint32_t p) {
-                          key[1 - a][d] = k;
-                          pos[1 - a][d] = (uint16_t)p;
-                      });
+        auto get = [&](int64_t first, uint32_t (&k)[4], uint32_t (&p)[4]) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = (int)first + u * 64 + (t & 63);
+                k[u] = i < shi ? key[a][i] : 0;
+                p[u] = i < shi ? pos[a][i] : 0;
+            }
+        };
+        uint32_t k[4], p[4];
+        get(slo, k, p);
+        place_segment(slo, shi, shift, digit_bits, next[w], k, p, get, [&](uint32_t d, uint32_t to_key, uint32_t to_pos) {
+            key[1 - a][d] = to_key;
+            pos[1 - a][d] = (uint16_t)to_pos;
+        });
         __syncthreads();
     }
     for (int i = t; i < n; i += SORT_NT) {
