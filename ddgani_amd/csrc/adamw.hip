@@ -191,7 +191,7 @@ struct AdwState {
 // A wave owns UNITS blocks of 256 elements, four consecutive elements per lane: every access is one contiguous piece per
 // wave, and a block's maximum is one reduction over the wave.  All loads come first.  Workgroups take the table from its end:
 // what the norm read last is still in the 256 MB cache, and in the wide variant everything but the gradients goes past it
-// (332 million elements 1 185 -> 1 112 us).  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
+// (332 million elements 1 185 -> 1 070 to 1 110 us, of which the norm takes 105).  SELF (with a clip, at most ADW_FEW workgroups in all): every workgroup
 // adds up the partial norms and forms the step's scalars itself, which is quicker than a launch of its own for them.
 // (One launch for norm and step, whose last workgroup to arrive goes on alone, is slower: an atomic that all XCDs share takes
 // 85 ns a workgroup.)

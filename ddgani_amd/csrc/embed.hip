@@ -124,7 +124,9 @@ extern "C" int ddg_embedding(const void *ids, int ids_64, int64_t n, const void 
 }
 
 // ---------------------------------------------------------------------------------------------
-// gradient: stable counting sort of (id, position), digits of at most 9 bits, least significant first
+// gradient: stable counting sort of (id, position), digits of at most 9 bits, least significant first.  Bound by latency: per pass 5
+// us for the counts and 8 (20 000 tokens) to 15 us (262 144) for the scatter, whose workgroups each add up the counts of all
+// tiles themselves instead of a third launch for them; up to 4 096 tokens 5 us in all
 // ---------------------------------------------------------------------------------------------
 #define SORT_NT 512
 #define SORT_WAVES (SORT_NT / 64)
@@ -355,7 +357,8 @@ __device__ __forceinline__ void add_rows(const float *__restrict__ src, const Co
 }
 
 // LEVEL 1: part[c] = sum of the dy rows of sorted positions [64 c, 64 c + 64) if they all belong to one row of the table;
-// LEVEL 2: part[c] = sum of the LEVEL-1 sums of [4 096 c, ...), under the same condition.  Other chunks are never read.
+// LEVEL 2: part[c] = sum of the LEVEL-1 sums of [4 096 c, ...), under the same condition.  Other chunks are never read.  Bound by
+// HBM (the rows of frequent ids among 262 144 tokens of 2 048 elements: 73 us), LEVEL 2 by latency (11 us).
 template <class T, int LEVEL, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
                                                       int64_t chunks, uint32_t V, const T *__restrict__ src, int64_t ld, int D,

@@ -18,11 +18,12 @@
 // and multiplied by v_mfma_f32_16x16x32_bf16 (8e-9 on the same data) at half the rate.
 //
 // Packed operand of `rows` rows and a reduction of `cols`: codes of colsp columns (cols rounded up to 128, zeros behind cols),
-// for the product's first operand row by row; for its second (weights, and X in dW) in pieces of 16 rows x 128 columns, [row /
-// 16][column / 128], as the matrix instruction takes them: lane r + 16 g holds codes 32 g to 32 g + 31 of row r, the first 16 of all
-// lanes come first.  A wave loads such a piece as 2 KB in a row.  (Rows up to the next multiple of 16 are zeros.)  Then from the next multiple of 256 bytes the scales as biased exponents (2^(e - 127)), four consecutive
-// blocks in one word: word [block / 4][row], byte block % 4.  The 16 rows of a matrix tile are 16 consecutive words.  1 KB
-// behind the scales belongs to the operand too: a workgroup reads whole 256-row pieces of them.
+// for the product's first operand row by row; for its second (weights, and X in dW) in pieces of 16 rows x 128 columns,
+// [row / 16][column / 128], as the matrix instruction takes them: lane r + 16 g holds codes 32 g to 32 g + 31 of row r, and the
+// first 16 of all lanes come first.  A wave loads such a piece as 2 KB in a row.  (Rows up to the next multiple of 16 are zeros.)
+// Then, from the next multiple of 256 bytes, the scales as biased exponents (2^(e - 127)), four consecutive blocks in one word:
+// word [block / 4][row], byte block % 4.  The 16 rows of a matrix tile are 16 consecutive words.  1 KB behind the scales belongs
+// to the operand too: a workgroup reads whole 256-row pieces of them.
 #include <type_traits>
 #include "types.h"
 
@@ -66,7 +67,8 @@ __device__ __forceinline__ void f8_put_scale(uint8_t *s, int64_t rows, int64_t r
 // ---------------------------------------------------------------------------------------------
 // packing
 // ---------------------------------------------------------------------------------------------
-// groups along the rows: 16 lanes x 8 elements hold a group, its maximum is a reduction over one DPP row
+// groups along the rows: 16 lanes x 8 elements hold a group, its maximum is a reduction over one DPP row.  Bound by HBM: 200 000 x
+// 176 fp32 37 us, 5.2 TB/s
 template <class T>
 __global__ __launch_bounds__(256) void k_f8_pack_rows(const T *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, uint8_t *q,
                                                       uint8_t *s) {
@@ -90,7 +92,9 @@ __global__ __launch_bounds__(256) void k_f8_pack_rows(const T *__restrict__ x, i
 // 128 x 128 tiles in registers, 8 x 8 elements per thread.  MODE F8_COLS: groups along the columns, packed transposed (qt, st);
 // F8_ROWS_COLS: those and groups along the rows (q, s); F8_TILE: one scale for the tile, packed both ways (qt may be NULL).
 // F8_ROWS_COLS packs a first operand (of either product), the others second operands.
-// sums (may be NULL): fp32 column sums of the tile, [row tile][cols].
+// sums (may be NULL): fp32 column sums of the tile, [row tile][cols].  Bound by HBM once there are a few tiles per CU (operands of
+// the gradients of 4001 x 2048 x 5000 in bf16 25 us, 4.2 TB/s), by latency below (128 x 176 x 352 7 us): hence all loads in front of
+// the first use, and the whole tile in registers.
 enum { F8_COLS, F8_ROWS_COLS, F8_TILE };
 struct F8Pack {
     const void *x;
@@ -264,7 +268,9 @@ __global__ __launch_bounds__(256) void k_f8_colsum(F8Colsum s) {
 // ---------------------------------------------------------------------------------------------
 // product of two packed operands: C[m, n] = sum over k of A[m, k] B[n, k]
 // ---------------------------------------------------------------------------------------------
-// A workgroup owns BM x BN of the result, a wave MT x NT tiles of 16 x 16; one block of the reduction is a stage.
+// A workgroup owns BM x BN of the result, a wave MT x NT tiles of 16 x 16; one block of the reduction is a stage.  With 256 x 256
+// the LDS (reads of 24 KB a wave and stage, copies of 64 KB) and the matrix unit are about equally long at work: 8192 x 4096 x 8192
+// 205 us, 2.7 PFLOP/s; larger tiles do not fit the registers (four waves of 128 x 128: 271 us then against 257).
 //
 // LDS image of a stage: B's pieces as they are packed, read by consecutive lanes at consecutive addresses.  A: rows of 128
 // bytes, whose eight 16-byte pieces are exchanged by f8_swap(row).  A 16-byte read is served
@@ -277,8 +283,8 @@ __global__ __launch_bounds__(256) void k_f8_colsum(F8Colsum s) {
 // One barrier per stage, towards its end: by then every fragment of stage k has been read, so its buffer takes stage k + 2,
 // and stage k + 1 has landed, whose fragments are read between the matrix instructions behind the barrier.  Codes: the wave holds
 // its NT fragments of B and takes those of A one after the other, two steps of NT instructions behind the barrier (the other
-// way round, 18 reads of 16 bytes fall into a quarter of the stage, more than the LDS delivers: 8192 x 4096 x 8192 256 us
-// against 248).  Expanded: it holds A and takes B, one column behind the barrier, so that B is expanded bit by bit
+// way round, 18 reads of 16 bytes fall into a quarter of the stage, more than the LDS delivers: 8192 x 4096 x 8192 with the
+// codes of X 234 us against 226).  Expanded: it holds A and takes B, one column behind the barrier, so that B is expanded bit by bit
 // (8192 x 4096 x 4096 235 us; the other way round 253).  The copies of a stage are issued one by one between the matrix
 // instructions: issued in a row they hold up the instructions behind them, as a CU takes about 64 bytes of them a cycle.
 template <int MT, int NT, int WM, int WN> struct F8Shape {
@@ -573,7 +579,7 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void k_f8_gemm_grads(F8Gemm d
     else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, dx_first ? id : id - nw);
 }
 
-// C = bias + sum of the parts, in their order; four columns per thread
+// C = bias + sum of the parts, in their order; four columns per thread.  Latency and HBM, 3.2 TB/s
 struct F8Join {
     const float *part;
     int64_t M, N;
@@ -747,8 +753,8 @@ static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
 // 352 x 176, a third more columns, 33.5 and 36.2).  A tile whose reduction
 // takes twice its share of all stages and more is split into parts of about that share (a whole number of scale words, so
 // four stages at least), which are added afterwards, where that saves more (0.6 us a stage) than it costs (a launch, 3 us, and
-// the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 13.7 us, 128 x 4096 x 4096
-// 36 -> 24 us; 256 x 1000 x 8192 would go from 16 to 21 us and is left whole.
+// the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 14 to 16 us, 128 x 4096 x
+// 4096 36 -> 24 us; 256 x 1000 x 8192 would go from 16 to 21 us and is left whole.
 static inline bool f8_wide(int64_t rows_a, int64_t rows_b) {
     const int64_t wide = ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256), small = ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128);
     return wide >= 192 && ceil_div64(wide, 256) * 3 < ceil_div64(small, F8_WORKGROUPS) * 2;
@@ -908,8 +914,8 @@ extern "C" int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t 
 
 // k_f8_skinny: X fits the LDS, and its quantisation by every workgroup (13 elements a ns, and 3 us a workgroup besides; one
 // workgroup per CU at a time) takes less than the detour over packed X and tiles, 18 us and with another result than bf16
-// 22 us.  Rows from which the tiles were quicker (bf16, in x out): 2048 x 2048 and 4096 x 4096 none, 8192 x 8192 nine, 14336 x 4096 thirteen, 4096 x 14336 six, 4096 x
-// 32000 one; 16 rows through 8192 x 8192 32 us here and 24 us there, through 4096 x 4096 10 and 14.
+// 22 us.  Rows from which the tiles were quicker (bf16, in x out): 2048 x 2048 and 4096 x 4096 none, 8192 x 8192 nine, 14336 x 4096
+// thirteen, 4096 x 14336 six, 4096 x 32000 one; 16 rows through 8192 x 8192 32 us here and 24 us there, through 4096 x 4096 10 and 14.
 static inline bool f8_skinny(int64_t rows, int64_t out, int64_t in, bool bf16) {
     const int64_t nk = f8_pad(in) / F8_BLOCK;
     return rows <= F8_SKINNY && rows * (nk * (F8_BLOCK + 1) + 16) <= F8_SKINNY_LDS &&
