@@ -552,8 +552,8 @@ template <int MT, int NT, int WM, int WN, bool EXPAND, class TO> __device__ __fo
         __builtin_memcpy(v, __builtin_assume_aligned(own + row * PITCH + (lane % LPR) * 16, 16), 16);
         TO *o = C + m * ldc + n;
         if (left == VEC) {
-            // (past the caches where results are large: they would not stay in them, and take 4 % less time)
-            if (MT * NT >= 16) store16_streaming(o, v);
+            // (past the caches where a wave writes whole lines of them: 4 to 12 % less time; not 64 columns of 16 bits, 10 % more)
+            if (MT * NT * sizeof(TO) >= 32) store16_streaming(o, v);
             else __builtin_memcpy(o, v, 16);
         } else {
 #pragma unroll
@@ -749,8 +749,9 @@ static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
 // cost less than those of 128 x 128 tiles (two per CU, two thirds of the time a round: 40 000 x 176 x 352 30.8 us with 256 x 256,
 // 25.3 with 128 x 128; 8192 x 4096 x 8192 is four rounds and eight); else 128 x 128, or 128 x 64 while
 // all tiles together have fewer than eight stages for each of 512 workgroups: there the time is latency.  Not where 128 x 128 tiles
-// come near one for each of those and cover no more columns (20 000 x 176 x 352 22.7 us with 128 x 64, 18.5 with 128 x 128; 40 000 x
-// 352 x 176, a third more columns, 33.5 and 36.2).  A tile whose reduction
+// come near one for each of those and cover no more columns (20 000 x 176 x 352 19.4 us with 128 x 64, 18.5 with 128 x 128); where
+// they cover more, 128 x 64 for fp32 results of short reductions and any number of rows (100 000 x 176 x 176 44.9 us and 48.9,
+// 100 000 x 1000 x 64 121 and 130, but 100 000 x 4096 x 64 506 and 494; 100 000 x 352 x 320 in bf16 67 and 56).  A tile whose reduction
 // takes twice its share of all stages and more is split into parts of about that share (a whole number of scale words, so
 // four stages at least), which are added afterwards, where that saves more (0.6 us a stage) than it costs (a launch, 3 us, and
 // the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 14 to 16 us, 128 x 4096 x
@@ -762,9 +763,10 @@ static inline bool f8_wide(int64_t rows_a, int64_t rows_b) {
 static inline int64_t f8_stages(int64_t rows_a, int64_t rows_b, int64_t cols, int bn) {
     return ceil_div64(rows_a, 128) * ceil_div64(rows_b, bn) * (f8_pad(cols) / F8_BLOCK);
 }
-static inline bool f8_narrow(int64_t rows_a, int64_t rows_b, int64_t cols) {
-    const bool many = ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128) >= 400 && ceil_div64(rows_b, 128) * 2 == ceil_div64(rows_b, 64);
-    return !many && f8_stages(rows_a, rows_b, cols, 128) < 8 * F8_WORKGROUPS;
+static inline bool f8_narrow(int64_t rows_a, int64_t rows_b, int64_t cols, bool f32) {
+    const bool latency = f8_stages(rows_a, rows_b, cols, 128) < 8 * F8_WORKGROUPS;
+    if (ceil_div64(rows_b, 128) * 2 != ceil_div64(rows_b, 64)) return latency || (f32 && f8_pad(cols) <= 8 * F8_BLOCK);
+    return latency && ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128) < 400;
 }
 struct F8Split {
     int64_t splits, blocks;
@@ -778,7 +780,7 @@ static inline F8Split f8_split(int64_t m, int64_t n, int64_t cols, int64_t all_s
 // the split of a product on its own
 static inline F8Split f8_split_one(int64_t rows_a, int64_t rows_b, int64_t cols, bool bf16) {
     if (bf16 && f8_wide(rows_a, rows_b)) return {1, ceil_div64(f8_pad(cols) / F8_BLOCK, 4) * 4};
-    const bool narrow = f8_narrow(rows_a, rows_b, cols);
+    const bool narrow = f8_narrow(rows_a, rows_b, cols, false);         // (short reductions are not split in either tile)
     return f8_split(rows_a, rows_b, cols, f8_stages(rows_a, rows_b, cols, narrow ? 64 : 128));
 }
 static inline size_t f8_parts_bytes(const F8Split &sp, int64_t m, int64_t n) {
@@ -816,7 +818,7 @@ static int f8_join_parts(const F8Join &a, int type, const F8Join &b, hipStream_t
 
 static int f8_gemm(const F8Operand &a, const F8Operand &b, const float *bias, void *c, int type, int64_t ldc, float *parts, hipStream_t s) {
     const F8Split sp = f8_split_one(a.rows, b.rows, a.cols, type == DDG_BF16);
-    const bool narrow = f8_narrow(a.rows, b.rows, a.cols);
+    const bool narrow = f8_narrow(a.rows, b.rows, a.cols, type == DDG_F32);
     auto go = [&](auto mt, auto nt, auto wm, auto wn, auto expand, auto to) {
         using TO = decltype(to);
         constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;

@@ -342,3 +342,12 @@ def test_few_rows_of_wide_layers(dev, M, K, N):
     x, W = data(M, K, 45, dev, BF16), data(N, K, 46, dev, BF16) * 0.02
     for ot in (F32, BF16):
         check_linear(x, W, None, ops.linear_fp8(x, ops.Fp8Weight(W), out_dtype=ot))
+
+
+@pytest.mark.parametrize("M,K,N", [(90001, 300, 176), (20001, 176, 352), (40001, 100, 352)])
+@pytest.mark.parametrize("ot", [F32, BF16, F16])
+def test_tall_layers(dev, M, K, N, ot):
+    """many rows of short reductions: every rule for the tiles' size"""
+    x, W = data(M, K, 47, dev), data(N, K, 48, dev) * 0.1
+    bias = torch.randn(N, generator=torch.Generator(device=dev).manual_seed(49), device=dev)
+    check_linear(x, W, bias, ops.linear_fp8(x, ops.Fp8Weight(W), bias=bias, out_dtype=ot))
