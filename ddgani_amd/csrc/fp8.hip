@@ -579,7 +579,10 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void k_f8_gemm_grads(F8Gemm d
     else f8_gemm_tile<4, NT, 2, 2, EXPAND, TO>(dx, dx_first ? id : id - nw);
 }
 
-// C = bias + sum of the parts, in their order; four columns per thread.  Latency and HBM, 3.2 TB/s
+// C = bias + sum of the parts, four columns per lane, in an order that the number of parts decides.  Up to eight parts: all of them
+// in flight, bound by HBM, 3.2 TB/s.  More: latency, so the waves of a workgroup share them (79 parts of 64 x 64 4.6 us, a
+// wave alone 9).
+#define F8_JOIN_ALONE 8
 struct F8Join {
     const float *part;
     int64_t M, N;
@@ -588,24 +591,47 @@ struct F8Join {
     void *C;
     int64_t ldc;
 };
-template <class TO> __device__ __forceinline__ void f8_join(const F8Join &j, int64_t i) {
-    const int64_t units = (j.N + 3) / 4, m = i / units, n = (i - m * units) * 4;
-    if (m >= j.M) return;
-    const int left = j.N - n < 4 ? (int)(j.N - n) : 4;
-    float v[4] = {}, p[4];
-    if (j.bias) load_n<4>(j.bias + n, left, v);
-#pragma unroll 4
-    for (uint32_t s = 0; s < j.splits; ++s) {
-        load_n<4>(j.part + (s * j.M + m) * j.N + n, left, p);
+template <class TO> __device__ __forceinline__ void f8_join(const F8Join &j, int64_t block, f32x4 (&lds)[4][64]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool alone = j.splits <= F8_JOIN_ALONE;
+    const int first = alone ? 0 : wave, step = alone ? 1 : 4;
+    const int64_t units = (j.N + 3) / 4, i = alone ? block * 256 + threadIdx.x : block * 64 + lane, m = i / units, n = (i - m * units) * 4;
+    const int left = m >= j.M ? 0 : j.N - n < 4 ? (int)(j.N - n) : 4;
+    const float *const part = j.part + (left ? m * j.N + n : 0);
+    f32x4 sum = {};
+    if (left == 4) {                                    // eight parts in flight (behind the end: the last one, not added)
+        for (uint32_t s = first; s < j.splits; s += 8 * step) {
+            float p[8][4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] += p[u];
+            for (int t = 0; t < 8; ++t) load_n<4>(part + (s + t * step < j.splits ? s + t * step : j.splits - 1) * j.M * j.N, 4, p[t]);
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                if (s + t * step < j.splits) sum += f32x4{p[t][0], p[t][1], p[t][2], p[t][3]};
+        }
+    } else {
+        for (uint32_t s = first; s < j.splits; s += step)
+#pragma unroll
+            for (int u = 0; u < 3; ++u)
+                if (u < left) sum[u] += part[s * j.M * j.N + u];
     }
+    if (!alone) {
+        lds[wave][lane] = sum;
+        __syncthreads();
+        if (wave) return;
+        sum = (lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]);
+    }
+    if (!left) return;
+    float v[4] = {};
+    if (j.bias) load_n<4>(j.bias + n, left, v);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] += sum[u];
     store_n<4>((TO *)j.C + m * j.ldc + n, left, v);
 }
 // a: of type TO, `first` workgroups; b: fp32 (either may be none)
 template <class TO> __global__ __launch_bounds__(256) void k_f8_join(F8Join a, uint32_t first, F8Join b) {
-    if (blockIdx.x < first) f8_join<TO>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
-    else f8_join<float>(b, (int64_t)(blockIdx.x - first) * 256 + threadIdx.x);
+    __shared__ f32x4 lds[4][64];
+    if (blockIdx.x < first) f8_join<TO>(a, blockIdx.x, lds);
+    else f8_join<float>(b, blockIdx.x - first, lds);
 }
 
 // Few rows, 16 at most (f8_skinny): bound by the bytes of B and by latency, so one launch does the layer.  A workgroup owns 16
@@ -754,8 +780,8 @@ static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
 // 100 000 x 1000 x 64 121 and 130, but 100 000 x 4096 x 64 506 and 494; 100 000 x 352 x 320 in bf16 67 and 56).  A tile whose reduction
 // takes twice its share of all stages and more is split into parts of about that share (a whole number of scale words, so
 // four stages at least), which are added afterwards, where that saves more (0.6 us a stage) than it costs (a launch, 3 us, and
-// the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 14 to 16 us, 128 x 4096 x
-// 4096 36 -> 24 us; 256 x 1000 x 8192 would go from 16 to 21 us and is left whole.
+// the parts written and read, 3.2 TB/s); all figures measured.  17 x 8192 x 1000 in fp32 53 -> 12.7 us, 128 x 4096 x 4096
+// 36 -> 21.5 us; 256 x 1000 x 8192 is left whole, 15 us.
 static inline bool f8_wide(int64_t rows_a, int64_t rows_b) {
     const int64_t wide = ceil_div64(rows_a, 256) * ceil_div64(rows_b, 256), small = ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128);
     return wide >= 192 && ceil_div64(wide, 256) * 3 < ceil_div64(small, F8_WORKGROUPS) * 2;
@@ -804,7 +830,7 @@ static F8Join f8_joined(const F8Operand &a, const F8Operand &b, const F8Split &s
                         int64_t ldc) {
     return {parts, a.rows, b.rows, (uint32_t)sp.splits, bias, c, ldc};
 }
-static inline int64_t f8_join_grid(const F8Join &j) { return j.splits > 1 ? ceil_div64(j.M * ((j.N + 3) / 4), 256) : 0; }
+static inline int64_t f8_join_grid(const F8Join &j) { return j.splits > 1 ? ceil_div64(j.M * ((j.N + 3) / 4), j.splits > F8_JOIN_ALONE ? 64 : 256) : 0; }
 // whichever of the two was split (b: fp32)
 static int f8_join_parts(const F8Join &a, int type, const F8Join &b, hipStream_t s) {
     const int64_t ga = f8_join_grid(a), gb = f8_join_grid(b);
