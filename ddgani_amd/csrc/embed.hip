@@ -406,6 +406,60 @@ __device__ __forceinline__ RowParts row_parts(uint32_t a, uint32_t b) {
 
 #define ROWS_MAX 32                   // table rows per wave, at most: one lane finds the positions of one row
 
+// Lane l: the first of n sorted keys that is >= v + min(l, rows), for l <= rows <= ROWS_MAX; by the whole wave (v and rows the same
+// in every lane).  64 probes at a time for the first and the last of them (two or three rounds of loads where a search by
+// halves needs 8 to 18, one after the other), then the few keys in between at once.
+__device__ __forceinline__ uint32_t wave_lower_bounds(const uint32_t *__restrict__ key, uint32_t n, uint32_t v, uint32_t rows) {
+    const uint32_t lane = threadIdx.x & 63, to[2] = {v, v + rows};
+    uint32_t lo[2] = {0, 0}, len[2] = {n, n};           // the place is in [lo, lo + len]
+    while (len[0] | len[1]) {
+        uint64_t less[2];
+        uint32_t step[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            step[i] = (len[i] + 63) / 64;
+            const uint32_t at = (lane + 1) * step[i] - 1;
+            less[i] = __ballot(at < len[i] && key[lo[i] + at] < to[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (!len[i]) continue;
+            const uint32_t skip = __popcll(less[i]) * step[i], left = len[i] > skip ? len[i] - skip : 0;
+            lo[i] += skip;
+            len[i] = left < step[i] - 1 ? left : step[i] - 1;
+        }
+    }
+    const uint32_t count = lo[1] - lo[0];
+    uint32_t x = lane < rows ? lane : rows;
+    if (count > 128) {                                  // frequent rows
+        uint32_t a = lo[0], b = lo[1];
+        while (__any(a < b)) {
+            const uint32_t mid = a + (b - a) / 2;
+            const bool go = a < b, is_less = go && key[mid] < v + x;
+            if (go && is_less) a = mid + 1;
+            if (go && !is_less) b = mid;
+        }
+        return a;
+    }
+    // how many of the keys are below, bit by bit from the top: `same` agree with x so far
+    uint32_t before = 0, d[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) d[i] = i * 64 + lane < count ? key[lo[0] + i * 64 + lane] - v : 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint64_t same = __ballot(i * 64 + lane < count), below = 0;
+#pragma unroll
+        for (int bit = 5; bit >= 0; --bit) {
+            const uint64_t ones = __ballot((d[i] >> bit) & 1);
+            if ((x >> bit) & 1) below |= same & ~ones;
+            same &= (x >> bit) & 1 ? ones : ~ones;
+        }
+        before += __popcll(below);
+    }
+    return lo[0] + before;
+}
+static_assert(ROWS_MAX < 64, "six bits");
+
 // A group of 2^lg lanes owns `rows` consecutive rows of the table and as many columns as it has lanes x 8.  The single tokens
 // of all its rows form one list, which is walked four at a time with the next four loads in flight, across the rows' borders:
 // most rows have few tokens, and a walk row by row would wait out the memory's latency for each of them (609 us, now
@@ -419,23 +473,28 @@ __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(co
     const int lane = threadIdx.x & 63, lanes = 1 << lg, in_group = lane & (lanes - 1), group = lane >> lg;
     const int64_t wave0 = ((int64_t)rblock * (EMB_NT / 64) + (threadIdx.x >> 6)) * ((64 >> lg) * rows);
     if (wave0 >= V) return;
-    // lane l: the first sorted position whose key is >= row wave0 + l
-    int64_t lo = 0, hi = n;
-    {
+    // lane l: where row wave0 + l begins, up to the one behind the wave's last
+    uint32_t begin;
+    if (rows > 1) {                                     // enough waves to hide a search by halves, which is less work (2 % of 500 us)
+        uint32_t lo = 0, hi = (uint32_t)n;
         const uint64_t v = wave0 + lane;
         while (__any(lo < hi)) {
-            const int64_t mid = (lo + hi) >> 1;
+            const uint32_t mid = lo + (hi - lo) / 2;
             const bool go = lo < hi, less = go && key[mid] < v;
             if (go && less) lo = mid + 1;
             if (go && !less) hi = mid;
         }
+        begin = lo;
+    } else {                                            // (65 536 tokens of 256 elements in 32 000 rows 63 -> 58 us)
+        const int here = V - wave0 < (64 >> lg) * rows ? (int)(V - wave0) : (64 >> lg) * rows;
+        begin = wave_lower_bounds(key, (uint32_t)n, (uint32_t)__builtin_amdgcn_readfirstlane((int)wave0), here);
     }
     const Columns c((slab * lanes + in_group) * EMB_VEC, D);
     const int64_t v0 = wave0 + group * rows;
     // lane r of the group: row r's positions and single tokens, and how many the rows up to it have.  From here on groups go
     // their own ways and exchange data within themselves only
     const int own = group * rows + (in_group < rows ? in_group : rows - 1);
-    const int first = __shfl((int)lo, own), behind = __shfl((int)lo, own + 1);
+    const int first = __shfl((int)begin, own), behind = __shfl((int)begin, own + 1);
     const RowParts rp = row_parts(first, behind);
     const int singles = in_group < rows && v0 + in_group < V ? (int)(rp.a1 - rp.a + rp.b - rp.b1) : 0;
     int upto = singles;                                 // inclusive prefix over the group's rows
