@@ -133,8 +133,13 @@ extern "C" int ddg_embedding(const void *ids, int ids_64, int64_t n, const void 
 #define SORT_BINS 512
 #define SORT_MAX_TILES 128            // a tile's workgroup reads every earlier tile's counts: 128 x 512 words at most
 #define SORT_SMALL 4096               // up to this many tokens one workgroup sorts in LDS
-#define CHUNK1 64
-#define CHUNK2 4096
+// Sums beforehand, of chunks of 2^lg1 positions and of 2^lg2: the longest walk that a row can need is 2 (2^lg1 - 1) single tokens, 2
+// (2^(lg2 - lg1) - 1) sums of 2^lg1 and n / 2^lg2 sums of 2^lg2
+struct Chunks {
+    int lg1, lg2;
+};
+#define SMALL_CHUNKS 65536
+static inline Chunks chunks_of(int64_t n) { return n <= SMALL_CHUNKS ? Chunks{4, 8} : Chunks{6, 12}; }
 
 struct SortPlan {
     int bits, passes, digit;          // id bits, number of passes, bits per pass
@@ -361,26 +366,26 @@ __device__ __forceinline__ void add_rows(const float *__restrict__ src, const Co
 // HBM (the rows of frequent ids among 262 144 tokens of 2 048 elements: 73 us), LEVEL 2 by latency (11 us).
 template <class T, int LEVEL, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
-                                                      int64_t chunks, uint32_t V, const T *__restrict__ src, int64_t ld, int D,
+                                                      int64_t chunks, Chunks ch, uint32_t V, const T *__restrict__ src, int64_t ld, int D,
                                                       float *__restrict__ part, int lg_tpr) {
     const int tpr = 1 << lg_tpr;
     const Columns cs((blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * EMB_VEC, D);
     const int64_t c = (int64_t)blockIdx.x * (EMB_NT >> lg_tpr) + (threadIdx.x >> lg_tpr);
-    const int len = LEVEL == 1 ? CHUNK1 : CHUNK2;
+    const int len = 1 << (LEVEL == 1 ? ch.lg1 : ch.lg2), adds = LEVEL == 1 ? len : 1 << (ch.lg2 - ch.lg1);
     if (c >= chunks || cs.col >= D) return;
     const uint32_t k = key[c * len];
     if (k >= V || k != key[c * len + len - 1]) return;
     float acc[EMB_VEC] = {};
     uint32_t p[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * 64 + u] : (uint32_t)(c * 64 + u);
-    for (int j = 0; j < 64; j += 8) {                   // eight rows in flight, and with them the next eight positions
+    for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * adds + u] : (uint32_t)(c * adds + u);
+    for (int j = 0; j < adds; j += 8) {                   // eight rows in flight, and with them the next eight positions
         vec8<T> v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = load_row<TINY, true>(src + (int64_t)p[u] * ld, cs);
-        const int next = j + 8 < 64 ? j + 8 : j;
+        const int next = j + 8 < adds ? j + 8 : j;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * 64 + next + u] : (uint32_t)(c * 64 + next + u);
+        for (int u = 0; u < 8; ++u) p[u] = LEVEL == 1 ? pos[c * adds + next + u] : (uint32_t)(c * adds + next + u);
 #pragma unroll
         for (int u = 0; u < 8; ++u) add_row<T>(acc, v[u]);
     }
@@ -392,13 +397,13 @@ __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict
 struct RowParts {
     uint32_t a, a1, a2, b2, b1, b;
 };
-__device__ __forceinline__ RowParts row_parts(uint32_t a, uint32_t b) {
+__device__ __forceinline__ RowParts row_parts(uint32_t a, uint32_t b, const Chunks &ch) {
     RowParts p = {a, b, b, b, b, b};
-    const uint32_t up1 = (a + CHUNK1 - 1) / CHUNK1 * CHUNK1, dn1 = b / CHUNK1 * CHUNK1;
+    const uint32_t up1 = (a + (1u << ch.lg1) - 1) >> ch.lg1 << ch.lg1, dn1 = b >> ch.lg1 << ch.lg1;
     if (up1 >= dn1) return p;                           // no whole chunk
     p.a1 = up1;
     p.b1 = dn1;
-    const uint32_t up2 = (a + CHUNK2 - 1) / CHUNK2 * CHUNK2, dn2 = b / CHUNK2 * CHUNK2;
+    const uint32_t up2 = (a + (1u << ch.lg2) - 1) >> ch.lg2 << ch.lg2, dn2 = b >> ch.lg2 << ch.lg2;
     p.a2 = up2 < dn2 ? up2 : dn1;
     p.b2 = up2 < dn2 ? dn2 : dn1;
     return p;
@@ -465,7 +470,7 @@ static_assert(ROWS_MAX < 64, "six bits");
 // most rows have few tokens, and a walk row by row would wait out the memory's latency for each of them (609 us, now
 // 398 us, for 262 144 tokens of 2 048 elements in 128 000 rows).
 template <class T, class TO, bool TINY>
-__global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n,
+__global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n, Chunks ch,
                                                       int64_t V, const T *__restrict__ dy, int64_t ld, int D,
                                                       const float *__restrict__ part1, const float *__restrict__ part2, float scale,
                                                       int accumulate, TO *__restrict__ out, int64_t ldo, int lg, int rows, int slabs, int stream) {
@@ -495,7 +500,7 @@ __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(co
     // their own ways and exchange data within themselves only
     const int own = group * rows + (in_group < rows ? in_group : rows - 1);
     const int first = __shfl((int)begin, own), behind = __shfl((int)begin, own + 1);
-    const RowParts rp = row_parts(first, behind);
+    const RowParts rp = row_parts(first, behind, ch);
     const int singles = in_group < rows && v0 + in_group < V ? (int)(rp.a1 - rp.a + rp.b - rp.b1) : 0;
     int upto = singles;                                 // inclusive prefix over the group's rows
     for (int d = 1; d < lanes; d <<= 1) {
@@ -510,11 +515,11 @@ __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(co
         const int64_t v = v0 + row;
         const uint32_t a = __shfl(first, row, lanes), b = __shfl(behind, row, lanes);
         if (v < V && c.col < D && !(accumulate && a == b)) {
-            const RowParts p = row_parts(a, b);
+            const RowParts p = row_parts(a, b, ch);
             if (p.a1 < p.b1) {
-                add_rows<TINY>(part1, c, p.a1 / CHUNK1, p.a2 / CHUNK1, acc);
-                add_rows<TINY>(part2, c, p.a2 / CHUNK2, p.b2 / CHUNK2, acc);
-                add_rows<TINY>(part1, c, p.b2 / CHUNK1, p.b1 / CHUNK1, acc);
+                add_rows<TINY>(part1, c, p.a1 >> ch.lg1, p.a2 >> ch.lg1, acc);
+                add_rows<TINY>(part2, c, p.a2 >> ch.lg2, p.b2 >> ch.lg2, acc);
+                add_rows<TINY>(part1, c, p.b2 >> ch.lg1, p.b1 >> ch.lg1, acc);
             }
             TO *o = out + v * ldo;
             vec8<TO> old = {};
@@ -542,7 +547,7 @@ __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(co
         for (int k = 0; k < rows; ++k) rr += __shfl(upto, k, lanes) <= it;
         const int rc = rr < rows ? rr : rows - 1;
         const uint32_t ordinal = it - (__shfl(upto, rc, lanes) - __shfl(singles, rc, lanes));
-        const RowParts p = row_parts(__shfl(first, rc, lanes), __shfl(behind, rc, lanes));
+        const RowParts p = row_parts(__shfl(first, rc, lanes), __shfl(behind, rc, lanes), ch);
         const uint32_t at = ordinal < p.a1 - p.a ? p.a + ordinal : p.b1 + (ordinal - (p.a1 - p.a));
         item_row = it < total ? rr : rows;
         item_pos = it < total ? (int)pos[at] : 0;
@@ -586,8 +591,9 @@ static inline EmbWs emb_carve(void *base, int64_t n, int D) {
         w.pos[i] = (uint32_t *)take((size_t)n * 4);
     }
     w.hist = (uint32_t *)take((size_t)SORT_MAX_TILES * SORT_BINS * 4);
-    w.part1 = (float *)take((size_t)(n / CHUNK1) * D * 4);
-    w.part2 = (float *)take((size_t)(n / CHUNK2) * D * 4);
+    const Chunks ch = chunks_of(n);
+    w.part1 = (float *)take((size_t)(n >> ch.lg1) * D * 4);
+    w.part2 = (float *)take((size_t)(n >> ch.lg2) * D * 4);
     w.bytes = o;
     return w;
 }
@@ -608,6 +614,7 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
     if (n > 0 && (!ids || !dy)) return DDG_E_ARG;
     if (!workspace || workspace_bytes < ddg_embedding_grad_workspace_bytes(n, D)) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 15) return DDG_E_ARG;
+    const Chunks ch = chunks_of(n);
     const int lg = emb_lg_tpr(D), rpb = EMB_NT >> lg;
     const int slabs = (D + (EMB_VEC << lg) - 1) / (EMB_VEC << lg);
     // k_embg_rows: groups of 8 to 64 lanes, and as many rows per group (16 at most, 32 per wave) as leave about 8 192 waves
@@ -617,7 +624,7 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
     const int most = ROWS_MAX / groups < 16 ? ROWS_MAX / groups : 16;
     rows = rows < 1 ? 1 : rows > most ? most : rows;
     const int64_t rgrid = ceil_div64(V, EMB_NT / 64 * groups * rows);
-    if (rgrid * rslabs > ddg_max_grid(EMB_NT) || ceil_div64(n / CHUNK1, rpb) > ddg_max_grid(EMB_NT)) return DDG_E_UNSUPPORTED;
+    if (rgrid * rslabs > ddg_max_grid(EMB_NT) || ceil_div64(n >> ch.lg1, rpb) > ddg_max_grid(EMB_NT)) return DDG_E_UNSUPPORTED;
     const EmbWs w = emb_carve(workspace, n, D);
     const SortPlan sp = sort_plan(n > 0 ? n : 1, V);
     const hipStream_t s = (hipStream_t)stream;
@@ -646,17 +653,17 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
         using TI = decltype(ti);
         auto sums = [&](auto tiny) {
             constexpr bool TINY = decltype(tiny)::value;
-            const int64_t c1 = n / CHUNK1, c2 = n / CHUNK2;
+            const int64_t c1 = n >> ch.lg1, c2 = n >> ch.lg2;
             if (c1)
                 k_embg_part<TI, 1, TINY><<<dim3((unsigned)ceil_div64(c1, rpb), slabs), EMB_NT, 0, s>>>(
-                    w.key[cur], w.pos[cur], c1, (uint32_t)V, (const TI *)dy, ld_dy, D, w.part1, lg);
+                    w.key[cur], w.pos[cur], c1, ch, (uint32_t)V, (const TI *)dy, ld_dy, D, w.part1, lg);
             if (c2)
                 k_embg_part<float, 2, TINY><<<dim3((unsigned)ceil_div64(c2, rpb), slabs), EMB_NT, 0, s>>>(
-                    w.key[cur], w.pos[cur], c2, (uint32_t)V, w.part1, D, D, w.part2, lg);
+                    w.key[cur], w.pos[cur], c2, ch, (uint32_t)V, w.part1, D, D, w.part2, lg);
             return ddg_with_type(out_type, [&](auto to) {
                 using TO = decltype(to);
                 k_embg_rows<TI, TO, TINY><<<(unsigned)(rgrid * rslabs), EMB_NT, 0, s>>>(
-                    w.key[cur], w.pos[cur], n, V, (const TI *)dy, ld_dy, D, w.part1, w.part2, scale, accumulate, (TO *)out, ld_out,
+                    w.key[cur], w.pos[cur], n, ch, V, (const TI *)dy, ld_dy, D, w.part1, w.part2, scale, accumulate, (TO *)out, ld_out,
                     rlg, (int)rows, (int)rslabs, V * D > EMB_STREAM);
                 DDG_CHECK_LAUNCH();
                 return (int)DDG_OK;
