@@ -7,9 +7,8 @@
 //
 // The gradient sorts the tokens instead of adding with atomics: (id, position) pairs go through a stable counting sort, so
 // every table row finds its positions in ascending order and is summed in registers, in one fixed order (bitwise
-// reproducible), and written once.  Frequent ids are long rows: sorted positions are cut into aligned chunks of 64, and a
-// chunk that belongs to ONE id is summed beforehand by k_embg_part (4 096-chunks of such sums by a second launch), so the
-// longest walk a row can need is 63 + 63 single tokens, 63 + 63 sums of 64 and n / 4 096 sums of 4 096.
+// reproducible), and written once.  Frequent ids are long rows: sorted positions are cut into aligned chunks (of 16, 32 or 64), and
+// a chunk that belongs to ONE id is summed beforehand by k_embg_part, chunks of 16, 32 or 64 such sums by a second launch.
 #include <type_traits>
 #include "types.h"
 
@@ -138,8 +137,11 @@ extern "C" int ddg_embedding(const void *ids, int ids_64, int64_t n, const void 
 struct Chunks {
     int lg1, lg2;
 };
-#define SMALL_CHUNKS 65536
-static inline Chunks chunks_of(int64_t n) { return n <= SMALL_CHUNKS ? Chunks{4, 8} : Chunks{6, 12}; }
+// Small ones where the walk's latency counts, larger ones where the number of the largest does.  Word-like ids: 5 000 tokens of 64
+// elements 31 us (with 64 and 4 096: 48), 65 536 of 256 73 (32 and 1 024: 80; 64 and 4 096: 92; but all of one id 117, 69 and 62),
+// 262 144 of 64 in 5 000 rows 79 (64 and 4 096: 99), 262 144 of 2 048 523 (538).  Fewer than 1 024 tokens: a second launch (3 us)
+// is dearer than 64 sums at most.
+static inline Chunks chunks_of(int64_t n) { return n < 1024 ? Chunks{4, 10} : n <= 65536 ? Chunks{4, 8} : n <= 1 << 20 ? Chunks{5, 10} : Chunks{6, 12}; }
 
 struct SortPlan {
     int bits, passes, digit;          // id bits, number of passes, bits per pass
@@ -361,8 +363,8 @@ __device__ __forceinline__ void add_rows(const float *__restrict__ src, const Co
     }
 }
 
-// LEVEL 1: part[c] = sum of the dy rows of sorted positions [64 c, 64 c + 64) if they all belong to one row of the table;
-// LEVEL 2: part[c] = sum of the LEVEL-1 sums of [4 096 c, ...), under the same condition.  Other chunks are never read.  Bound by
+// LEVEL 1: part[c] = sum of the dy rows of the c-th 2^lg1 sorted positions if they all belong to one row of the table;
+// LEVEL 2: part[c] = sum of the LEVEL-1 sums of the c-th 2^lg2 positions, under the same condition.  Other chunks are never read.  Bound by
 // HBM (the rows of frequent ids among 262 144 tokens of 2 048 elements: 73 us), LEVEL 2 by latency (11 us).
 template <class T, int LEVEL, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
@@ -392,8 +394,8 @@ __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict
     store_row<TINY>(part + c * D, cs, acc);
 }
 
-// How the sorted positions [a, b) of a row divide: single tokens [a, a1) and [b1, b), sums of 64 [a1, a2) and [b2, b1), sums
-// of 4 096 [a2, b2)
+// How the sorted positions [a, b) of a row divide: single tokens [a, a1) and [b1, b), sums of 2^lg1 [a1, a2) and [b2, b1), sums
+// of 2^lg2 [a2, b2)
 struct RowParts {
     uint32_t a, a1, a2, b2, b1, b;
 };
