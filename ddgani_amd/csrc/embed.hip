@@ -365,7 +365,7 @@ __device__ __forceinline__ void add_rows(const float *__restrict__ src, const Co
 
 // LEVEL 1: part[c] = sum of the dy rows of the c-th 2^lg1 sorted positions if they all belong to one row of the table;
 // LEVEL 2: part[c] = sum of the LEVEL-1 sums of the c-th 2^lg2 positions, under the same condition.  Other chunks are never read.  Bound by
-// HBM (the rows of frequent ids among 262 144 tokens of 2 048 elements: 73 us), LEVEL 2 by latency (11 us).
+// HBM (the rows of frequent ids among 262 144 tokens of 2 048 elements: 87 us), LEVEL 2 by latency (7 us).
 template <class T, int LEVEL, bool TINY>
 __global__ __launch_bounds__(EMB_NT) void k_embg_part(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
                                                       int64_t chunks, Chunks ch, uint32_t V, const T *__restrict__ src, int64_t ld, int D,
@@ -470,7 +470,7 @@ static_assert(ROWS_MAX < 64, "six bits");
 // A group of 2^lg lanes owns `rows` consecutive rows of the table and as many columns as it has lanes x 8.  The single tokens
 // of all its rows form one list, which is walked four at a time with the next four loads in flight, across the rows' borders:
 // most rows have few tokens, and a walk row by row would wait out the memory's latency for each of them (609 us, now
-// 398 us, for 262 144 tokens of 2 048 elements in 128 000 rows).
+// 370 us, for 262 144 tokens of 2 048 elements in 128 000 rows).
 template <class T, class TO, bool TINY>
 __global__ __launch_bounds__(EMB_NT, sizeof(T) == 2 ? 5 : 4) void k_embg_rows(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n, Chunks ch,
                                                       int64_t V, const T *__restrict__ dy, int64_t ld, int D,
