@@ -9,12 +9,19 @@
 // launch (the table of at most 64 tensors travels in the kernel arguments, so a captured graph holds it); the step number,
 // the bias corrections and the clip factor live in device memory, so a replayed graph advances them.
 //
-// 8-bit states: blocks of 256 consecutive elements share an fp32 scale s = max / 448 and keep e4m3 codes.  m is rounded to
-// nearest.  What is kept of v is its root r: the root halves the exponent range a block has to span, 2^-9 ... 448 = 2^17.8
-// in r is 2^35 in v.  b2 close to 1 changes r by less than half a code per step, which rounding to nearest would undo each
-// time, so r is rounded up where its fraction plus a dither number passes one.  The number is a Weyl sequence over (element,
-// step): it needs no random generator and no memory, and over the steps it is equally often above as below any fraction.
-// A positive r is never stored as 0, so that no element divides by eps alone.
+// 8-bit states: blocks of 256 consecutive elements share an fp32 scale s = max / 448 and keep e4m3 codes.  What is kept of v is its
+// root r: the root halves the exponent range a block has to span, 2^-9 ... 448 = 2^17.8 in r is 2^35 in v.  Both averages are slow:
+// where a step changes one by less than half a code, rounding to nearest puts the code back that was there, in every step.  b2
+// close to 1 does that to r everywhere, so r is rounded up where its fraction plus a dither number passes one.  The number is a Weyl
+// sequence over (element, step): it needs no random generator and no memory, and over the steps it is equally often above as below
+// any fraction.  A positive r is never stored as 0, so that no element divides by eps alone.
+// m must not keep its code either once its gradient stops: r goes on falling beside it, and the weight would walk on m / r for ever
+// (b1 0.9, b2 0.95, half of every block without a gradient: 2 000 steps moved that half by 686 lr where 32 bits move it by 2.5).
+// In e4m3's normal range half a code is 1/16 of the value at most, so that up to b1 = 0.93 a decay of 1 - b1 always reaches the next
+// code and nearest, which is less noise than a dither, is kept there; in the linear range below 2^-6 (codes under 8: 0.9 x 4 = 3.6 is 4
+// again) m is rounded by a dither of its own, as r is but down to 0, and above b1 = 0.93 everywhere.  The same half: moved by 2.5 lr, and
+// then it rests.  What nearest still costs is the last half code of a gradient that stays the same: m comes to a stop up to half a
+// code / (1 - b1) from it.
 #include <math.h>
 #include <type_traits>
 #include "types.h"
@@ -26,6 +33,8 @@
 #define ADW_TABLE 64
 #define ADW_FEW 1024                              // workgroups that sum all partial norms themselves, at most
 #define ADW_NORM_GRID 2048                        // workgroups of the norm per launch: eight per CU, 16 KB of partial sums
+#define ADW_NEAREST_B1 0.93                       // 1 - b1 above half a code, 1/16 of a value, with room for the roundings of m / s
+#define ADW_LINEAR 0.015625f                      // 2^-6: codes below are multiples of 2^-9
 #define ADW_TINY 7.888609052210118e-31f           // 2^-100: blocks below are stored as zeros (448 / max stays finite)
 
 struct AdwEntry {
@@ -43,7 +52,7 @@ static_assert(ADW_TABLE == 64, "one lane looks at one entry");
 
 struct AdwScalars {
     float step_size, root2;                       // lr / (1 - b1^t), sqrt(1 - b2^t)
-    uint32_t dither;                              // of the step
+    uint32_t dither_m, dither_r;                  // of the step
 };
 // device side of the handle (DDG_ADAMW_CONTROL_BYTES)
 struct AdwControl {
@@ -56,6 +65,7 @@ struct AdwControl {
 struct AdwHyper {
     double lr, b1, b2;
     float max_norm;                               // <= 0: no clip
+    float m_low;                                  // 8 bits: m that was and is below this (in units of the scale) is dithered
 };
 
 __device__ __forceinline__ double adw_power(double b, int64_t t) {
@@ -66,7 +76,8 @@ __device__ __forceinline__ double adw_power(double b, int64_t t) {
 }
 // bias corrections in fp64, as a host would form them
 __device__ __forceinline__ AdwScalars adw_scalars(const AdwHyper &h, int64_t t) {
-    return {(float)(h.lr / (1.0 - adw_power(h.b1, t))), (float)sqrt(1.0 - adw_power(h.b2, t)), (uint32_t)t * 2246822507u};
+    return {(float)(h.lr / (1.0 - adw_power(h.b1, t))), (float)sqrt(1.0 - adw_power(h.b2, t)), (uint32_t)t * 2447445413u,
+            (uint32_t)t * 2246822507u};
 }
 
 // the tensor of a workgroup: the last entry whose chunk0 <= chunk, one entry per lane
@@ -145,24 +156,37 @@ __device__ __forceinline__ float wave_max(float x) {
     return fmaxf(x, __shfl_xor(x, 32));
 }
 
-// four non-negative values (already divided by the scale) -> e4m3 codes.  The bits below the code's last are the fraction
+// a non-negative value (already divided by the scale) -> e4m3 code, u below 2^20.  The bits below the code's last are the fraction
 // within the code's step; below 2^-6 the codes are linear, which adding 2^-6 turns into the same case.
-__device__ __forceinline__ uint32_t encode_dithered(const float (&y)[ADW_VEC], uint32_t first, uint32_t dither) {
+__device__ __forceinline__ int code_dithered(float y, uint32_t u) {
+    const bool small = y < ADW_LINEAR;
+    return (int)((__builtin_bit_cast(uint32_t, small ? y + ADW_LINEAR : y) + u) >> 20) - (small ? 968 : 960);
+}
+__device__ __forceinline__ uint32_t encode_r(const float (&y)[ADW_VEC], uint32_t first, uint32_t dither) {
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < ADW_VEC; ++i) {
-        const bool small = y[i] < 0.015625f;
-        const uint32_t u = ((first + i) * 2654435769u + dither) >> 12;
-        int c = (int)((__builtin_bit_cast(uint32_t, small ? y[i] + 0.015625f : y[i]) + u) >> 20) - (small ? 968 : 960);
+        int c = code_dithered(y[i], ((first + i) * 2654435769u + dither) >> 12);
         c = c < 1 ? 1 : c > 126 ? 126 : c;
         if (!(y[i] > 0.f)) c = y[i] == 0.f ? 0 : 127;             // NaN stays NaN
         w |= (uint32_t)c << (8 * i);
     }
     return w;
 }
-__device__ __forceinline__ uint32_t encode_nearest(const float (&y)[ADW_VEC]) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+// old: what was stored, in units of the new scale.  (The Weyl steps of the two dithers have nothing in common: 2^32 times the
+// inverse of the golden ratio and its like for x^3 = x + 1)
+__device__ __forceinline__ uint32_t encode_m(const float (&y)[ADW_VEC], const float (&old)[ADW_VEC], float low, uint32_t first,
+                                             uint32_t dither) {
+    uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)w, true);
+#pragma unroll
+    for (int i = 0; i < ADW_VEC; ++i) {
+        const float a = fabsf(y[i]);
+        int c = code_dithered(a, ((first + i) * 3242174889u + dither) >> 12);
+        c = (c > 126 ? 126 : c) | (y[i] < 0.f ? 128 : 0);
+        if (a < low && fabsf(old[i]) < low) w = (w & ~(0xFFu << (8 * i))) | (uint32_t)c << (8 * i);       // (never a NaN)
+    }
+    return w;
 }
 __device__ __forceinline__ void decode(uint32_t w, float scale, float (&y)[ADW_VEC]) {
     y[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0) * scale;
@@ -286,8 +310,12 @@ __global__ __launch_bounds__(ADW_NT) void k_adamw(AdwTable tb, AdwState st, AdwC
                 m[k] = m[k] * im;
                 r[k] = r[k] * ir;
             }
-            store_codes<WIDE>((uint8_t *)st.m + f, n, encode_nearest(m));
-            store_codes<WIDE>((uint8_t *)st.v + f, n, encode_dithered(r, (uint32_t)f, sc.dither));
+            float old[ADW_VEC];
+            const float grown = ms[u] * im;                       // the block's largest m before / now
+            decode(mc[u], grown, old);
+            // (a block that has no m yet, or one that grows by half in a step, holds no slow average)
+            store_codes<WIDE>((uint8_t *)st.m + f, n, encode_m(m, old, grown > 0.6667f ? h.m_low : 0.f, (uint32_t)f, sc.dither_m));
+            store_codes<WIDE>((uint8_t *)st.v + f, n, encode_r(r, (uint32_t)f, sc.dither_r));
             if (lane == 0) {
                 st.ms[blk] = top_m >= ADW_TINY ? top_m * (1.f / 448.f) : 0.f;
                 st.vs[blk] = top_r >= ADW_TINY ? top_r * (1.f / 448.f) : 0.f;
@@ -372,7 +400,7 @@ extern "C" int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, in
     AdwControl *ctl = (AdwControl *)control;
     static_assert(sizeof(AdwControl) <= DDG_ADAMW_CONTROL_BYTES, "control block");
     double *part = (double *)workspace;
-    const AdwHyper h = {lr, beta1, beta2, (float)max_norm};
+    const AdwHyper h = {lr, beta1, beta2, (float)max_norm, beta1 <= ADW_NEAREST_B1 ? ADW_LINEAR : INFINITY};
     const bool wide = adw_wide(tensors, n_tensors), clip = max_norm > 0;
     const int64_t total = adw_total(tensors, n_tensors, wide);
     const bool self = clip && !wide && total > 0;       // no k_adamw_begin

@@ -561,8 +561,9 @@ int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const void *dy, i
  * multiple of DDG_ADAMW_BLOCK, and tensors do not overlap in them.
  * state_bits 32: exp_avg, exp_avg_sq fp32 (m, v); the scales are not read.
  * state_bits 8: e4m3 codes of m and of sqrt(v), one fp32 scale for every DDG_ADAMW_BLOCK elements
- *   (scale[offset / DDG_ADAMW_BLOCK + block]); value = code * scale.  m to nearest; sqrt(v) by a
- *   dither that is a function of (element, step), so that equal calls give equal bits.
+ *   (scale[offset / DDG_ADAMW_BLOCK + block]); value = code * scale.  sqrt(v) is rounded by a
+ *   dither that is a function of (element, step), so that equal calls give equal bits; m to nearest where that keeps the
+ *   decay by b1 (b1 <= 0.93: codes of 8 and more), else by such a dither too, so that a weight whose gradient stops comes to rest.
  * masters (may be NULL): fp32 weights of the 16-bit parameters, flat like the states; the parameter
  *   becomes the rounding of its master.  fp32 parameters do not use it.
  * control: DDG_ADAMW_CONTROL_BYTES of device memory, zeroed by the caller before the first step: int64 step count at byte 0,
