@@ -769,10 +769,11 @@ def embedding(ids, table, scale: float = 1.0, out_dtype: Optional[torch.dtype] =
 
 
 def embedding_grad(ids, dy, n_rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
-                   out_dtype: torch.dtype = torch.float32, out=None, accumulate: bool = False):
+                   out_dtype: Optional[torch.dtype] = None, out=None, accumulate: bool = False):
     """ddg_embedding_grad: the gradient of ``embedding`` in its table, [n_rows, D]: row v is scale * the sum of dy over the
     tokens with id v (zeros if there is none).  dy [*ids.shape, D].  Ids outside [0, n_rows) and padding_idx have no gradient.
-    accumulate: adds to ``out`` and leaves rows that no token names as they are.  Equal calls give equal bits."""
+    out_dtype: of the result (default: that of ``out``, else float32).  accumulate: adds to ``out`` and leaves rows that no token
+    names as they are.  Equal calls give equal bits."""
     ip, i64 = _ids(ids)
     n, D = ids.numel(), dy.shape[-1]
     if dy.shape != (*ids.shape, D) and dy.shape != (n, D):
@@ -783,9 +784,9 @@ def embedding_grad(ids, dy, n_rows: int, scale: float = 1.0, padding_idx: Option
     if out is None:
         if accumulate:
             raise _lib.DdgError("embedding_grad: accumulate needs out")
-        out = dy.new_empty((n_rows, D), dtype=out_dtype)
-    elif out.shape != (n_rows, D):
-        raise _lib.DdgError(f"embedding_grad: out {tuple(out.shape)}, expected {(n_rows, D)}")
+        out = dy.new_empty((n_rows, D), dtype=out_dtype or torch.float32)
+    elif out.shape != (n_rows, D) or (out_dtype is not None and out.dtype != out_dtype):
+        raise _lib.DdgError(f"embedding_grad: out is {out.dtype} {tuple(out.shape)}, expected {out_dtype or ''} {(n_rows, D)}")
     op, ldo = _matrix(out, "out")
     dev = dy.get_device()
     stream = _on(dev, ids, out)
