@@ -400,7 +400,9 @@ extern "C" int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, in
     AdwControl *ctl = (AdwControl *)control;
     static_assert(sizeof(AdwControl) <= DDG_ADAMW_CONTROL_BYTES, "control block");
     double *part = (double *)workspace;
-    const AdwHyper h = {lr, beta1, beta2, (float)max_norm, beta1 <= ADW_NEAREST_B1 ? ADW_LINEAR : INFINITY};
+    // (a positive max_norm below the smallest fp32 number still clips)
+    const float to_norm = max_norm > 0 ? fmaxf((float)max_norm, 1.401298464e-45f) : 0.f;
+    const AdwHyper h = {lr, beta1, beta2, to_norm, beta1 <= ADW_NEAREST_B1 ? ADW_LINEAR : INFINITY};
     const bool wide = adw_wide(tensors, n_tensors), clip = max_norm > 0;
     const int64_t total = adw_total(tensors, n_tensors, wide);
     const bool self = clip && !wide && total > 0;       // no k_adamw_begin

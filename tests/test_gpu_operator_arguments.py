@@ -26,3 +26,16 @@ def test_embedding_grad_refuses_an_out_of_another_type(dev):
     assert ops.embedding_grad(ids, dy.to(BF16), 4).dtype == F32
     assert ops.embedding_grad(ids, dy, 4, out=out.to(BF16)).dtype == BF16
     assert ops.embedding_grad(ids, dy, 4, out_dtype=F32, out=out) is out
+
+
+@pytest.mark.parametrize("n", [500, 1_100_003])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_clips_to_a_norm_below_the_smallest_float(dev, n, bits):
+    """max_norm = 1e-50: the clip factor is 1e-50 / |g|, below every fp32 number, for small and for large nets; so the gradients
+    count as zeros (g' < 1e-38 where |g| >= 1: an update of lr g' / eps < 1e-32) and the weights stay but for their decay"""
+    w = torch.ones(n, device=dev)
+    opt = ops.AdamW([w], [torch.full((n,), 0.5, device=dev)], lr=1e-2, weight_decay=0.5, max_norm=1e-50, state_bits=bits)
+    norm = opt.step()
+    assert abs(float(norm) - 0.5 * n ** 0.5) <= 1e-6 * float(norm)
+    assert torch.equal(w, torch.full((n,), 1 - 1e-2 * 0.5, device=dev)) and int(opt.step_count) == 1
+    assert float(opt.exp_avg.float().abs().max()) <= 1e-38
