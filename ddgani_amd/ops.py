@@ -5,6 +5,7 @@ pointers of contiguous tensors to libddgani_hip.so on torch's current HIP stream
 """
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 import functools
 import os
@@ -916,6 +917,7 @@ class AdamW:
         spans = sorted((_ptr(p), p.numel() * p.element_size()) for p in self.params if p.numel())
         if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
             raise _lib.DdgError("AdamW: parameters share memory")
+        self._starts, self._ends = [a for a, _ in spans], [a + n for a, n in spans]
         self.offsets, total = [], 0
         for p in self.params:
             self.offsets.append(total)
@@ -956,6 +958,10 @@ class AdamW:
                 raise _lib.DdgError(f"AdamW: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
         ptr = [(_ptr(g), _type(g, "grads")) for g in grads]
         _on(self.dev, *grads)
+        for (a, _), g in zip(ptr, grads):                    # the last parameter that begins in front of the gradient's end
+            last = bisect.bisect_left(self._starts, a + g.numel() * g.element_size()) - 1
+            if g.numel() and last >= 0 and self._ends[last] > a:
+                raise _lib.DdgError("AdamW: a gradient shares memory with a parameter")
         for t, (p, code) in zip(self._t, ptr):
             t.grad, t.grad_type = p, code
         self.grads = grads

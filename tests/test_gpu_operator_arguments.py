@@ -39,3 +39,20 @@ def test_adamw_clips_to_a_norm_below_the_smallest_float(dev, n, bits):
     assert abs(float(norm) - 0.5 * n ** 0.5) <= 1e-6 * float(norm)
     assert torch.equal(w, torch.full((n,), 1 - 1e-2 * 0.5, device=dev)) and int(opt.step_count) == 1
     assert float(opt.exp_avg.float().abs().max()) <= 1e-38
+
+
+def test_adamw_refuses_gradients_inside_parameters(dev):
+    """a step writes the parameters while it reads the gradients"""
+    buf = torch.zeros(1000, device=dev)
+    params = [buf[600:700], buf[100:300], torch.zeros(0, device=dev)]
+    fine = [torch.zeros(100, device=dev), torch.zeros(200, device=dev), torch.zeros(0, device=dev)]
+    for bad in ([buf[600:700], fine[1]], [buf[650:750], fine[1]], [buf[501:601], fine[1]], [fine[0], buf[299:499]],
+                [buf[200:300], fine[1]], [fine[0], buf[50:250]]):
+        with pytest.raises(DdgError):
+            ops.AdamW(params, bad + fine[2:])
+    beside = [buf[500:600], buf[300:500], buf[150:150]]
+    opt = ops.AdamW(params, beside)
+    opt.step()
+    with pytest.raises(DdgError):
+        opt.set_grads([buf[699:799]] + beside[1:])
+    assert opt.grads[0] is beside[0]
