@@ -353,10 +353,14 @@ static int adw_check(const ddg_adamw_tensor *t, int n_tensors, int64_t state_len
 // counts), else four blocks per wave
 static inline bool adw_wide(const ddg_adamw_tensor *t, int n_tensors) { return adw_total(t, n_tensors, false) > ADW_FEW; }
 
+static inline int64_t adw_parts(const ddg_adamw_tensor *t, int n_tensors) {
+    const int64_t parts = adw_total(t, n_tensors, adw_wide(t, n_tensors));
+    return parts > 0 ? parts : 1;
+}
 extern "C" size_t ddg_adamw_workspace_bytes(const ddg_adamw_tensor *tensors, int n_tensors) {
     if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return 0;
-    const int64_t parts = adw_total(tensors, n_tensors, adw_wide(tensors, n_tensors));
-    return (size_t)(parts > 0 ? parts : 1) * sizeof(double);
+    const int64_t parts = adw_parts(tensors, n_tensors);
+    return (size_t)(parts > ADW_FEW || !adw_wide(tensors, n_tensors) ? parts : ADW_FEW) * sizeof(double);     // (what fewer elements take)
 }
 
 // calls f(table, workgroups) for groups of at most ADW_TABLE non-empty tensors that `take` accepts, in their order
@@ -411,7 +415,7 @@ extern "C" int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, in
     for (int i = 0; i < n_tensors; ++i)
         if (tensors[i].numel > 0) types |= 1u << (tensors[i].param_type * 3 + tensors[i].grad_type);
     if (clip) {
-        if (!workspace || workspace_bytes < ddg_adamw_workspace_bytes(tensors, n_tensors)) return DDG_E_WORKSPACE;
+        if (!workspace || workspace_bytes < adw_parts(tensors, n_tensors) * sizeof(double)) return DDG_E_WORKSPACE;
         for (int gt = DDG_F32; gt <= DDG_F16; ++gt) {
             if (!(types & (0x49u << gt))) continue;
             const int r = adw_groups(

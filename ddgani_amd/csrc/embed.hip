@@ -141,7 +141,10 @@ struct Chunks {
 // elements 31 us (with 64 and 4 096: 48), 65 536 of 256 73 (32 and 1 024: 80; 64 and 4 096: 92; but all of one id 117, 69 and 62),
 // 262 144 of 64 in 5 000 rows 79 (64 and 4 096: 99), 262 144 of 2 048 523 (538).  Fewer than 1 024 tokens: a second launch (3 us)
 // is dearer than 64 sums at most.
-static inline Chunks chunks_of(int64_t n) { return n < 1024 ? Chunks{4, 10} : n <= 65536 ? Chunks{4, 8} : n <= 1 << 20 ? Chunks{5, 10} : Chunks{6, 12}; }
+static constexpr int64_t CHUNKS_SMALL = 65536, CHUNKS_MIDDLE = 1 << 20;
+static inline Chunks chunks_of(int64_t n) {
+    return n < 1024 ? Chunks{4, 10} : n <= CHUNKS_SMALL ? Chunks{4, 8} : n <= CHUNKS_MIDDLE ? Chunks{5, 10} : Chunks{6, 12};
+}
 
 struct SortPlan {
     int bits, passes, digit;          // id bits, number of passes, bits per pass
@@ -602,7 +605,12 @@ static inline EmbWs emb_carve(void *base, int64_t n, int D) {
 
 extern "C" size_t ddg_embedding_grad_workspace_bytes(int64_t n, int D) {
     if (n < 0 || n > 0x7FFFFFFF || D < 1 || D > EMB_MAX_D) return 0;
-    return emb_carve(nullptr, n, D).bytes;
+    size_t most = emb_carve(nullptr, n, D).bytes;       // fewer tokens may need more: larger chunks begin behind these
+    for (const int64_t last : {CHUNKS_SMALL, CHUNKS_MIDDLE}) {
+        const size_t bytes = emb_carve(nullptr, n < last ? n : last, D).bytes;
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const void *dy, int dy_type, int64_t ld_dy, int64_t V,
@@ -614,7 +622,7 @@ extern "C" int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const 
     if (n > 0x7FFFFFFF || V > 0x7FFFFFFE) return DDG_E_UNSUPPORTED;
     if (n == 0 && accumulate) return DDG_OK;
     if (n > 0 && (!ids || !dy)) return DDG_E_ARG;
-    if (!workspace || workspace_bytes < ddg_embedding_grad_workspace_bytes(n, D)) return DDG_E_WORKSPACE;
+    if (!workspace || workspace_bytes < emb_carve(nullptr, n, D).bytes) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 15) return DDG_E_ARG;
     const Chunks ch = chunks_of(n);
     const int lg = emb_lg_tpr(D), rpb = EMB_NT >> lg;

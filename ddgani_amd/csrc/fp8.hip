@@ -797,20 +797,44 @@ static inline bool f8_narrow(int64_t rows_a, int64_t rows_b, int64_t cols, bool 
 struct F8Split {
     int64_t splits, blocks;
 };
-static inline F8Split f8_split(int64_t m, int64_t n, int64_t cols, int64_t all_stages) {
-    const int64_t nk = f8_pad(cols) / F8_BLOCK, share = ceil_div64(ceil_div64(all_stages, F8_WORKGROUPS), 4) * 4;
-    const int64_t splits = ceil_div64(nk, share);
-    if (nk < 2 * share || (nk - share) * 600 < 3000 + splits * m * n / 800) return {1, ceil_div64(nk, 4) * 4};
-    return {splits, share};
+static inline F8Split f8_share(int64_t cols, int64_t all_stages) {
+    const int64_t share = ceil_div64(ceil_div64(all_stages, F8_WORKGROUPS), 4) * 4;
+    return {ceil_div64(f8_pad(cols) / F8_BLOCK, share), share};
 }
-// the split of a product on its own
+// the largest m whose split saves more than it costs (0: none)
+static inline int64_t f8_split_most(int64_t n, int64_t cols, const F8Split &sp) {
+    const int64_t nk = f8_pad(cols) / F8_BLOCK, saved = (nk - sp.blocks) * 600 - 3000;         // ns
+    return nk < 2 * sp.blocks || saved < 0 ? 0 : ((saved + 1) * 800 - 1) / (sp.splits * n);
+}
+static inline F8Split f8_split(int64_t m, int64_t n, int64_t cols, int64_t all_stages) {
+    const F8Split sp = f8_share(cols, all_stages);
+    if (m > f8_split_most(n, cols, sp)) return {1, ceil_div64(f8_pad(cols) / F8_BLOCK, 4) * 4};
+    return sp;
+}
+// stages and split of a product on its own (short reductions are not split in either tile)
+static inline int64_t f8_stages_one(int64_t rows_a, int64_t rows_b, int64_t cols) {
+    return f8_stages(rows_a, rows_b, cols, f8_narrow(rows_a, rows_b, cols, false) ? 64 : 128);
+}
 static inline F8Split f8_split_one(int64_t rows_a, int64_t rows_b, int64_t cols, bool bf16) {
     if (bf16 && f8_wide(rows_a, rows_b)) return {1, ceil_div64(f8_pad(cols) / F8_BLOCK, 4) * 4};
-    const bool narrow = f8_narrow(rows_a, rows_b, cols, false);         // (short reductions are not split in either tile)
-    return f8_split(rows_a, rows_b, cols, f8_stages(rows_a, rows_b, cols, narrow ? 64 : 128));
+    return f8_split(rows_a, rows_b, cols, f8_stages_one(rows_a, rows_b, cols));
 }
 static inline size_t f8_parts_bytes(const F8Split &sp, int64_t m, int64_t n) {
     return sp.splits > 1 ? ((size_t)sp.splits * m * n * 4 + 255) & ~(size_t)255 : 0;
+}
+// The most that the parts of a product with up to m rows take: stages(rows) depends on the number of row tiles alone, so that for each
+// number the largest m that is split counts.  None is split above 256 tiles (two shares would be more than the reduction)
+template <class Stages> static inline size_t f8_parts_most(int64_t m, int64_t n, int64_t cols, const Stages &stages) {
+    size_t most = 0;
+    for (int64_t t = 1; (t - 1) * 128 < m && t * ceil_div64(n, 128) <= 256; ++t) {
+        const int64_t rows = t * 128 < m ? t * 128 : m;
+        const F8Split sp = f8_share(cols, stages(rows));
+        const int64_t split = f8_split_most(n, cols, sp), last = rows < split ? rows : split;
+        if (last <= (t - 1) * 128) continue;
+        const size_t bytes = f8_parts_bytes(sp, last, n);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 template <class S>
@@ -878,13 +902,16 @@ struct F8GradSplits {
     bool apart, narrow;                 // two launches (dx in 256 x 256 tiles); 128 x 64 tiles
     F8Split dx, dw;
 };
+static inline int64_t f8_grad_stages(int64_t rows, int64_t out, int64_t in, int bn) {
+    return f8_stages(rows, in, out, bn) + f8_stages(out, in, rows, bn);
+}
+static inline bool f8_grad_narrow(int64_t rows, int64_t out, int64_t in) { return f8_grad_stages(rows, out, in, 128) < 8 * F8_WORKGROUPS; }
 static inline F8GradSplits f8_grad_splits(int64_t rows, int64_t out, int64_t in, bool bf16) {
     F8GradSplits g;
     const int64_t tw = ceil_div64(out, 128) * ceil_div64(in, 128);
     g.apart = bf16 && f8_wide(rows, in) && out > 1024 && tw * 4 >= ceil_div64(tw, F8_WORKGROUPS) * F8_WORKGROUPS * 3;
-    g.narrow = f8_stages(rows, in, out, 128) + f8_stages(out, in, rows, 128) < 8 * F8_WORKGROUPS;
-    const int bn = g.narrow ? 64 : 128;
-    const int64_t all = f8_stages(rows, in, out, bn) + f8_stages(out, in, rows, bn);
+    g.narrow = f8_grad_narrow(rows, out, in);
+    const int64_t all = f8_grad_stages(rows, out, in, g.narrow ? 64 : 128);
     g.dx = g.apart ? f8_split_one(rows, in, out, bf16) : f8_split(rows, in, out, all);
     g.dw = g.apart ? f8_split_one(out, in, rows, false) : f8_split(out, in, rows, all);
     return g;
@@ -954,7 +981,7 @@ extern "C" size_t ddg_fp8_linear_workspace_bytes(int64_t rows, int64_t out, int6
     if (!f8_dims_ok(rows, in) || !f8_dims_ok(out, 0) || in < 1 || out < 1) return 0;
     if (f8_skinny(rows, out, in, true)) return 0;
     // (the result's type decides about more rows there, and about 256 x 256 tiles, which are not split: room for either)
-    return ddg_fp8_operand_bytes(rows, in) + f8_parts_bytes(f8_split_one(rows, out, in, false), rows, out);
+    return ddg_fp8_operand_bytes(rows, in) + f8_parts_most(rows, out, in, [&](int64_t m) { return f8_stages_one(m, out, in); });
 }
 
 extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t rows, const void *packed_w, int64_t out, int64_t in,
@@ -989,7 +1016,8 @@ extern "C" int ddg_fp8_linear(const void *x, int x_type, int64_t ld_x, int64_t r
                 return nk > 8 ? go(Int<16>()) : go(Int<8>());
             });
         });
-    if (!workspace || workspace_bytes < ddg_fp8_linear_workspace_bytes(rows, out, in)) return DDG_E_WORKSPACE;
+    const size_t parts = f8_parts_bytes(f8_split_one(rows, out, in, y_type == DDG_BF16), rows, out);
+    if (!workspace || workspace_bytes < ddg_fp8_operand_bytes(rows, in) + parts) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 255) return DDG_E_ARG;
     const F8Operand a = f8_operand(workspace, rows, in);
     const int rc = f8_pack_rows(x, x_type, ld_x, a, s);
@@ -1001,7 +1029,8 @@ struct F8GradWs {
     float *sums, *parts_dx, *parts_dw;
     size_t bytes;
 };
-static inline F8GradWs f8_grad_carve(void *base, int64_t rows, int64_t out, int64_t in) {
+// parts_dx, parts_dw: bytes of the parts of the two products
+static inline F8GradWs f8_grad_carve(void *base, int64_t rows, int64_t out, int64_t in, size_t parts_dx, size_t parts_dw) {
     char *p = (char *)base;
     size_t o = 0;
     auto take = [&](size_t b) {
@@ -1014,21 +1043,19 @@ static inline F8GradWs f8_grad_carve(void *base, int64_t rows, int64_t out, int6
     w.dyt = take(ddg_fp8_operand_bytes(out, rows));
     w.xt = take(ddg_fp8_operand_bytes(in, rows));
     w.sums = (float *)take((size_t)ceil_div64(rows, F8_BLOCK) * out * 4);
-    size_t px = 0, pw = 0;                              // (either way that dx's type may have them done)
-    for (int bf16 = 0; bf16 < 2; ++bf16) {
-        const F8GradSplits sp = f8_grad_splits(rows, out, in, bf16);
-        const size_t x = f8_parts_bytes(sp.dx, rows, in), y = f8_parts_bytes(sp.dw, out, in);
-        px = x > px ? x : px;
-        pw = y > pw ? y : pw;
-    }
-    w.parts_dx = (float *)take(px);
-    w.parts_dw = (float *)take(pw);
+    w.parts_dx = (float *)take(parts_dx);
+    w.parts_dw = (float *)take(parts_dw);
     w.bytes = o;
     return w;
 }
 extern "C" size_t ddg_fp8_linear_grads_workspace_bytes(int64_t rows, int64_t out, int64_t in) {
-    if (!f8_dims_ok(rows, in) || !f8_dims_ok(out, 0) || out < 1 || in < 1) return 0;
-    return f8_grad_carve(nullptr, rows, out, in).bytes;
+    if (!f8_dims_ok(rows, in) || !f8_dims_ok(out, 0) || in < 1 || out < 1) return 0;
+    // Where the products go apart nothing is split: dX is 256 x 256 tiles, and two shares of dW's 384 tiles and more are longer than
+    // its reduction.  Together both have the same number of stages, so that dW's share is 1 / 256 of them at least
+    const size_t dx = f8_parts_most(rows, in, out, [&](int64_t m) { return f8_grad_stages(m, out, in, f8_grad_narrow(m, out, in) ? 64 : 128); });
+    const int64_t nk = ceil_div64(rows, F8_BLOCK), tw = f8_tiles(out, in), few = ceil_div64(nk, 4), share = ceil_div64(256, tw);
+    const size_t dw = nk < 8 || tw > 128 ? 0 : f8_parts_bytes({few < share ? few : share, 4}, out, in);
+    return f8_grad_carve(nullptr, rows, out, in, dx, dw).bytes;
 }
 
 extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, const void *x, int x_type, int64_t ld_x,
@@ -1039,9 +1066,10 @@ extern "C" int ddg_fp8_linear_grads(const void *dy, int dy_type, int64_t ld_dy, 
         ((uintptr_t)packed_wt & 255))
         return DDG_E_ARG;
     if (!f8_product_ok(rows, in, out) || !f8_product_ok(out, in, rows)) return DDG_E_UNSUPPORTED;
-    if (!workspace || workspace_bytes < ddg_fp8_linear_grads_workspace_bytes(rows, out, in)) return DDG_E_WORKSPACE;
+    const F8GradSplits sp = f8_grad_splits(rows, out, in, dx_type == DDG_BF16);
+    const F8GradWs w = f8_grad_carve(workspace, rows, out, in, f8_parts_bytes(sp.dx, rows, in), f8_parts_bytes(sp.dw, out, in));
+    if (!workspace || workspace_bytes < w.bytes) return DDG_E_WORKSPACE;
     if ((uintptr_t)workspace & 255) return DDG_E_ARG;
-    const F8GradWs w = f8_grad_carve(workspace, rows, out, in);
     const hipStream_t s = (hipStream_t)stream;
     const F8Operand gy = f8_operand(w.dy, rows, out), gyt = f8_operand(w.dyt, out, rows), xt = f8_operand(w.xt, in, rows);
     const int64_t tiles_dy = f8_tiles(rows, out), tiles_x = f8_tiles(rows, in), row_tiles = ceil_div64(rows, F8_BLOCK);

@@ -543,6 +543,7 @@ int ddg_decode_table(const float *code, const uint8_t *m, const double *obs, con
  * an order that depends on the arguments alone: equal calls give equal bits.  With accumulate, rows
  * that no id names are left as they are; without, they become zero.
  * D <= 2^26, V <= 2^31 - 1 (gradient: 2^31 - 2), n <= 2^31 - 1 (gradient).  out overlaps no input.
+ * A workspace of the size for n serves every smaller n.
  * ------------------------------------------------------------------------------------- */
 int ddg_embedding(const void *ids, int ids_64, int64_t n, const void *table, int table_type, int64_t V, int D,
                   int64_t ld_table, float scale, void *out, int out_type, int64_t ld_out, void *stream);
@@ -571,7 +572,7 @@ int ddg_embedding_grad(const void *ids, int ids_64, int64_t n, const void *dy, i
  *   so a captured graph may be replayed.  If the norm is not finite nothing changes but `norm`.
  *   (Squares are formed in fp32: so does a gradient above 1.8e19.)  Without a clip a gradient that is not finite reaches the state, in 8 bits that of its whole block.
  * tensors: HOST array, read before the call returns; weight_decay >= 0.  Parameters and gradients do not overlap.
- *   workspace: only for max_norm > 0.
+ *   workspace: only for max_norm > 0; one for these tensors serves fewer and shorter ones.
  * ------------------------------------------------------------------------------------- */
 #define DDG_ADAMW_BLOCK 256
 #define DDG_ADAMW_CONTROL_BYTES 64
@@ -605,7 +606,7 @@ int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, int state_bit
  * 2^22 tiles of 128 x 128, else DDG_E_UNSUPPORTED.  Results overlap no input.
  * Packed operand [rows, cols]: ddg_fp8_operand_bytes(rows, cols) bytes, aligned to 256.
  * ddg_fp8_pack_weight: W -> packed [out, in] and, for the gradients, packed_t [in, out] (may be NULL).
- * db may be NULL.  A workspace is aligned to 256.
+ * db may be NULL.  A workspace is aligned to 256; one of the size for `rows` serves fewer rows.
  * ------------------------------------------------------------------------------------- */
 size_t ddg_fp8_operand_bytes(int64_t rows, int64_t cols);
 int ddg_fp8_pack_weight(const void *W, int type, int64_t ld, int64_t out, int64_t in, void *packed, void *packed_t,

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from ddgani_amd import ops
+from ddgani_amd import _lib, ops
 from ddgani_amd._lib import DdgError
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,32 @@ def test_adamw_refuses_gradients_inside_parameters(dev):
     with pytest.raises(DdgError):
         opt.set_grads([buf[699:799]] + beside[1:])
     assert opt.grads[0] is beside[0]
+
+
+def test_a_workspace_for_the_largest_call_serves_smaller_ones(dev):
+    """the last batch of an epoch: fewer tokens or rows than the workspace was sized for, which take other chunks and splits"""
+    L, gen = _lib.lib(), torch.Generator(device=dev).manual_seed(1)
+    stream = torch.cuda.current_stream().cuda_stream
+    D, V = 64, 100
+    ws = torch.empty(L.ddg_embedding_grad_workspace_bytes(70000, D), dtype=torch.uint8, device=dev)
+    for n in (70000, 65537, 65536, 1024, 1023, 3):
+        ids, dy = torch.randint(0, V, (n,), generator=gen, device=dev), torch.randn(n, D, generator=gen, device=dev)
+        out = torch.empty(V, D, device=dev)
+        assert L.ddg_embedding_grad(ids.data_ptr(), 1, n, dy.data_ptr(), 0, D, V, D, 1.0, -1, 0, out.data_ptr(), 0, D, ws.data_ptr(),
+                                    ws.numel(), stream) == 0
+        assert torch.equal(out, ops.embedding_grad(ids, dy, V))
+    inn = outd = 4096
+    W = ops.Fp8Weight(torch.randn(outd, inn, generator=gen, device=dev))
+    ws = torch.empty(L.ddg_fp8_linear_workspace_bytes(600, outd, inn), dtype=torch.uint8, device=dev)
+    wg = torch.empty(L.ddg_fp8_linear_grads_workspace_bytes(600, outd, inn), dtype=torch.uint8, device=dev)
+    for rows in (600, 512, 128, 17, 1):
+        for dt, code in ((F32, 0), (BF16, 1)):
+            x, dy = (torch.randn(rows, k, generator=gen, device=dev).to(dt) for k in (inn, outd))
+            y, dx, dw = (torch.empty(s, dtype=t, device=dev) for s, t in (((rows, outd), dt), ((rows, inn), dt), ((outd, inn), F32)))
+            assert L.ddg_fp8_linear(x.data_ptr(), code, inn, rows, W.packed.data_ptr(), outd, inn, None, y.data_ptr(), code, outd,
+                                    ws.data_ptr(), ws.numel(), stream) == 0
+            assert L.ddg_fp8_linear_grads(dy.data_ptr(), code, outd, x.data_ptr(), code, inn, rows, W.packed_t.data_ptr(), outd, inn,
+                                          dx.data_ptr(), code, inn, dw.data_ptr(), None, wg.data_ptr(), wg.numel(), stream) == 0
+            assert torch.equal(y, ops.linear_fp8(x, W))
+            for a, b in zip((dx, dw), ops.linear_fp8_grads(dy, x, W)):
+                assert torch.equal(a, b)
