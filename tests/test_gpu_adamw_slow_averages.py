@@ -82,9 +82,10 @@ def test_weights_follow_a_gradient_far_below_a_code(dev, betas):
 
 @pytest.mark.parametrize("b1", [0.9, 0.95])
 def test_codes_of_m(dev, b1):
-    """b1 = 0.9: nearest, but the dithered code for what was and is in the linear range; b1 = 0.95: dithered everywhere; either
-    only where the block's largest m grew by less than half.  From the stored state in 64 bits; what lies within 1e-4 of a border may go either way (a value in units of a
-    code, up to 16 of them, is off by 16 x 60 x 2^-24 = 6e-5)."""
+    """b1 = 0.9: nearest, but the dithered code where the old code and the nearest one are linear (below 2^-6); b1 = 0.95:
+    dithered everywhere; either only where the block's largest m grew by less than half.  From the stored state in 64 bits; what
+    lies within 1e-4 of a border may go either way (a value in units of a code, up to 16 of them, is off by 16 x 60 x 2^-24 =
+    6e-5)."""
     n = 5000
     gen = torch.Generator(device=dev).manual_seed(2)
     g = (torch.rand(n, generator=gen, device=dev) * 40 - 31).exp2() * 4e4       # 2^-31 ... 2^9, times 4e4; smaller or larger each step
@@ -95,22 +96,19 @@ def test_codes_of_m(dev, b1):
         spread = lambda: opt.exp_avg_scale.double().repeat_interleave(256)[:n]
         m0, s0 = opt.exp_avg.float().double()[:n] * spread(), spread()
         opt.step()
-        y, old = (b1 * m0 + (1 - b1) * g.double()) / spread(), m0 / spread()
+        y, old = (b1 * m0 + (1 - b1) * g.double()) / spread(), m0.abs() / s0.clamp(min=1e-300)
         grid = torch.exp2(torch.frexp(y.abs().clamp(min=2.0 ** -6))[1].double() - 4)
         u = ((torch.arange(n, device=dev) * 3242174889 + t * 2447445413) % 2 ** 32).double() / 2 ** 32
         low = torch.floor(y.abs() / grid)
         frac = y.abs() / grid - low
-        low_range = float("inf") if b1 > 0.93 else 2.0 ** -6
-        grown = s0 / spread()
-        by_dither = (grown > 0.6667) & (y.abs() < low_range) & (old.abs() < low_range)
-        want = torch.where(by_dither, low + (frac + u >= 1), torch.round(y.abs() / grid)) * grid
+        grown, nearest = s0 / spread(), torch.round(y.abs() / grid) * grid
+        by_dither = (grown > 0.6667) & ((nearest < 2.0 ** -6) & (old < 2.0 ** -6) | torch.tensor(b1 > 0.93, device=dev))
+        want = torch.where(by_dither, (low + (frac + u >= 1)) * grid, nearest)
         want = want.clamp(max=448.0) * torch.sign(y)
-        border = torch.where(by_dither, ((frac + u - 1).abs() < 1e-4) | ((frac < 1e-4) & (low > 0)) | (frac > 1 - 1e-4),
-                             (frac - 0.5).abs() < 1e-4)
-        border |= ((y.abs() / 2.0 ** -6 - 1).abs() < 1e-4) | ((old.abs() / 2.0 ** -6 - 1).abs() < 1e-4)
-        border |= (grown / 0.6667 - 1).abs() < 1e-4
+        border = ((frac - 0.5).abs() < 1e-4) | ((grown / 0.6667 - 1).abs() < 1e-4)
+        border |= by_dither & (((frac + u - 1).abs() < 1e-4) | ((frac < 1e-4) & (low > 0)) | (frac > 1 - 1e-4))
         got = opt.exp_avg.float().double()[:n]
         assert torch.equal(got[~border], want[~border]), t
         assert border.float().mean() < 0.02
-        dithered += int((by_dither & (want.abs() != (torch.round(y.abs() / grid) * grid)) & ~border).sum())
+        dithered += int((by_dither & (want.abs() != nearest) & ~border).sum())
     assert dithered > 100
