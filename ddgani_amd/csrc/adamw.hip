@@ -175,7 +175,8 @@ __device__ __forceinline__ uint32_t encode_r(const float (&y)[ADW_VEC], uint32_t
 }
 // was: the codes stored so far.  every: all are dithered, else those that are linear codes (no exponent) before and now, in a branch
 // that most waves pass by (nearest alone 1 081 us for the step of 332 million elements, 1 102 so; every lane through it 1 112 and
-// 1 138 on another card, and small steps 8 % longer).  (The Weyl steps of the two dithers have nothing in common: 2^32 times the inverse of the golden ratio and its like for x^3 = x + 1)
+// 1 138 on another card, and small steps 8 % longer).  (The Weyl steps of the two dithers have nothing in common: 2^32 times the
+// inverse of the golden ratio and its like for x^3 = x + 1)
 __device__ __forceinline__ uint32_t encode_m(const float (&y)[ADW_VEC], uint32_t was, bool every, uint32_t first, uint32_t dither) {
     uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)w, true);

@@ -764,8 +764,9 @@ static inline int64_t f8_tiles(int64_t rows, int64_t cols) { return ceil_div64(r
 
 #define F8_WORKGROUPS 512                               // two per CU
 // Reductions are addressed with 32-bit offsets within a workgroup's 256 rows; both gradients' tiles and db's workgroups (at
-// most two for a tile of dW) fit one launch of 256 threads each.  Tiles of 128 x 64 and splits: only where there are fewer than
-// eight stages for each of F8_WORKGROUPS.  Checked in front of an entry point's first launch.
+// most two for a tile of dW) fit one launch of 256 threads each.  Tiles of 128 x 64 are at most twice as many: 2^23 for a product on its
+// own, and both gradients take them only below eight stages for each of F8_WORKGROUPS; splits are of products of up to 256 tiles.
+// Checked in front of an entry point's first launch.
 #define F8_MAX_REDUCTION ((int64_t)1 << 24)
 static inline bool f8_product_ok(int64_t rows_a, int64_t rows_b, int64_t cols) {
     return f8_pad(cols) < F8_MAX_REDUCTION && ceil_div64(rows_a, 128) * ceil_div64(rows_b, 128) < (1 << 22);

@@ -7,7 +7,6 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
 static inline bool ddg_type_ok(int t) { return t == DDG_F32 || t == DDG_BF16 || t == DDG_F16; }
-static inline int ddg_type_bytes(int t) { return t == DDG_F32 ? 4 : 2; }
 
 // workgroups that a launch takes at most: it counts its threads in 32 bits
 static inline int64_t ddg_max_grid(int threads) { return 0xFFFFFFFFll / threads; }
