@@ -138,8 +138,8 @@ struct Chunks {
     int lg1, lg2;
 };
 // Small ones where the walk's latency counts, larger ones where the number of the largest does.  Word-like ids: 5 000 tokens of 64
-// elements 31 us (with 64 and 4 096: 48), 65 536 of 256 73 (32 and 1 024: 80; 64 and 4 096: 92; but all of one id 117, 69 and 62),
-// 262 144 of 64 in 5 000 rows 79 (64 and 4 096: 99), 262 144 of 2 048 523 (538).  Fewer than 1 024 tokens: a second launch (3 us)
+// elements 31 us (with 64 and 4 096: 48), 65 536 of 256 73 (32 and 1 024: 80; 64 and 4 096: 92), of eight ids 61 (71; 112), of
+// 200 50 (51; 71), but all of one id 117, 69 and 62: its row's n / 2^lg2 sums are added by one group of lanes; 262 144 of 64 in 5 000 rows 79 (64 and 4 096: 99), 262 144 of 2 048 523 (538).  Fewer than 1 024 tokens: a second launch (3 us)
 // is dearer than 64 sums at most.
 static constexpr int64_t CHUNKS_SMALL = 65536, CHUNKS_MIDDLE = 1 << 20;
 static inline Chunks chunks_of(int64_t n) {

@@ -14,7 +14,8 @@
 // The fp8 matrix instructions drop bits inside: they align a group of products to its largest before adding them, which
 // leaves 1.4e-5 of a result's size for one block and, as the cuts add up, 2e-4 for a sum over 32 blocks (measured against
 // exact sums of normal codes).  That is far below the rounding of a bf16 result (2e-3) but not below that of an fp16 or fp32
-// one, so only bf16 results come from them; for the others the codes are expanded to bf16, which holds code x scale exactly,
+// one, so only bf16 results come from them (where large products of a
+// block cancel, what is dropped can be more than the small result's rounding: another result type avoids it); for the others the codes are expanded to bf16, which holds code x scale exactly,
 // and multiplied by v_mfma_f32_16x16x32_bf16 (8e-9 on the same data) at half the rate.
 //
 // Packed operand of `rows` rows and a reduction of `cols`: codes of colsp columns (cols rounded up to 128, zeros behind cols),
@@ -268,9 +269,10 @@ __global__ __launch_bounds__(256) void k_f8_colsum(F8Colsum s) {
 // ---------------------------------------------------------------------------------------------
 // product of two packed operands: C[m, n] = sum over k of A[m, k] B[n, k]
 // ---------------------------------------------------------------------------------------------
-// A workgroup owns BM x BN of the result, a wave MT x NT tiles of 16 x 16; one block of the reduction is a stage.  With 256 x 256
-// the LDS (reads of 24 KB a wave and stage, copies of 64 KB) and the matrix unit are about equally long at work: 8192 x 4096 x 8192
-// 205 us, 2.7 PFLOP/s; larger tiles do not fit the registers (four waves of 128 x 128: 271 us then against 257).
+// A workgroup owns BM x BN of the result, a wave MT x NT tiles of 16 x 16; one block of the reduction is a stage.  256 x 256, 8192 x
+// 4096 x 8192: 205 us and 2.7 PFLOP/s in a long run (225 us in the first ten calls, while the clock settles).  Of a stage's 3 290
+// cycles the matrix unit is at work for 2 048, the LDS for 1 070 with reads (24 KB a wave; conflicts 50) and for some 1 000 with
+// copies (64 KB), by counters; larger tiles do not fit the registers (four waves of 128 x 128: 271 us then against 257).
 //
 // LDS image of a stage: B's pieces as they are packed, read by consecutive lanes at consecutive addresses.  A: rows of 128
 // bytes, whose eight 16-byte pieces are exchanged by f8_swap(row).  A 16-byte read is served

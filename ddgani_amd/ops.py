@@ -749,7 +749,8 @@ def _ids(ids: torch.Tensor):
 def embedding(ids, table, scale: float = 1.0, out_dtype: Optional[torch.dtype] = None, out=None):
     """ddg_embedding: scale * table[ids] -> [*ids.shape, D].  ids int32 / int64, contiguous; table [V, D] float32, bfloat16 or
     float16 with contiguous rows (a row stride is fine).  An id outside [0, V) -- the -1 of a padded batch -- gives zeros.
-    out_dtype: of the result (default: the table's); out: a contiguous tensor, or a matrix [ids.numel(), D] with a row stride."""
+    out_dtype: of the result (default: the table's); out: a contiguous tensor, or a matrix [ids.numel(), D] with a row stride.
+    As everywhere in this module there is no autograd: the table's gradient is ``embedding_grad``."""
     ip, i64 = _ids(ids)
     tp, ld = _matrix(table, "table")
     V, D = table.shape
@@ -825,7 +826,10 @@ class Fp8Weight:
 
 def linear_fp8(x, weight: Fp8Weight, bias=None, out_dtype: Optional[torch.dtype] = None, out=None):
     """ddg_fp8_linear: x [rows, in] times the packed weight, + bias (float32 [out]) -> [rows, out] in out_dtype (default: x's).
-    x is quantised within the call, in groups of 128 along its rows; few rows (up to 16) take one launch."""
+    x is quantised within the call, in groups of 128 along its rows.  Up to 16 rows take one launch with exact products where
+    quantising x in every workgroup costs less than a launch for it (16 rows of 4096 x 4096, nine of 8192 x 8192, none of
+    4096 x 32000); all others are packed first, and bf16 results then drop bits below about 2^-14 of a block's largest product
+    (out_dtype=torch.float32 does not).  A lookup's result goes in as y.view(-1, D)."""
     xp, ld = _matrix(x, "x")
     rows, inn = x.shape
     outd = weight.out_dim

@@ -600,8 +600,11 @@ int ddg_adamw_step(const ddg_adamw_tensor *tensors, int n_tensors, int state_bit
  * A block's scale is the smallest power of two that brings its largest magnitude to 448 or below;
  * a block whose largest magnitude is below 2^-100 counts as zeros.  An infinity or a NaN gives NaN where
  * it is multiplied; beside an infinity the finite elements of its block count as zeros.
- * Products of bf16 results drop bits below about 2^-14 of a block's largest product, far below the
- * result's rounding; all other results are sums of exact products in fp32.
+ * Products of bf16 results drop bits below about 2^-14 of a block's largest product: far below the rounding of a
+ * result of that size, but not of a small one that is left where large products of a block cancel.  All other results, and dW, are
+ * sums of exact products in fp32; so are bf16 results of up to 16 rows where (rows in / 13 + 3000) max(out, 4096) <= 73.7 million and
+ * rows in <= 140 000, about (other results: 90.1 million): they take one launch and no workspace.  A layer's bits thus depend on its
+ * number of rows and its result's type.
  * Reductions (in; out and rows for the gradients) shorter than 2^24, X of fewer than 2^35 elements and results of fewer than
  * 2^22 tiles of 128 x 128, else DDG_E_UNSUPPORTED.  Results overlap no input.
  * Packed operand [rows, cols]: ddg_fp8_operand_bytes(rows, cols) bytes, aligned to 256.
